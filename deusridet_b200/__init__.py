@@ -4,3 +4,4 @@ declared in include/drkv.h.  This package is the thin Python host used by the te
 benchmark; the product is libdrkv.so."""
 from .capi import DrkvError, Geometry, Config, load_library  # noqa: F401
 from .engine import PagedKVEngine  # noqa: F401
+from .rope import Rope  # noqa: F401

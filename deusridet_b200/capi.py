@@ -51,6 +51,18 @@ class EvictRecord(C.Structure):
     _fields_ = [("kind", C.c_int32), ("seq", C.c_int32), ("logical", C.c_int32), ("page", C.c_int32)]
 
 
+class RopeConfig(C.Structure):
+    _fields_ = [("head_dim", C.c_int32), ("rotary_dim", C.c_int32), ("layout", C.c_int32), ("dtype", C.c_int32),
+                ("scaling", C.c_int32), ("device", C.c_int32), ("original_context", C.c_int32),
+                ("low_freq_factor", C.c_float), ("high_freq_factor", C.c_float), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float), ("attention_factor", C.c_float), ("theta", C.c_double), ("factor", C.c_double)]
+
+
+class RopeRows(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("heads", C.c_int32), ("src_token_stride", C.c_int64),
+                ("src_head_stride", C.c_int64), ("dst_token_stride", C.c_int64), ("dst_head_stride", C.c_int64)]
+
+
 _vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
 _pi32 = C.POINTER(C.c_int32)
 
@@ -150,6 +162,10 @@ SIGNATURES = {
     "drkv_k_decode_scratch_bytes": (_sz, [C.POINTER(Geometry), _i]),
     "drkv_k_decode_kernel_error": (_i, [_vp, _vp]),
     "drkv_k_decode_attention_noalloc": (_i, [C.POINTER(Geometry), _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp]),
+    "drkv_rope_create": (_i, [C.POINTER(RopeConfig), C.POINTER(_vp)]),
+    "drkv_rope_destroy": (None, [_vp]),
+    "drkv_rope_frequencies": (_i, [_vp, C.POINTER(C.c_double), _i]),
+    "drkv_rope_apply": (_i, [_vp, _i, _vp, C.POINTER(RopeRows), C.POINTER(RopeRows), _i, _vp]),
 }
 NOALLOC_SCRATCH_BYTES = 4 << 20
 

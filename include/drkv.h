@@ -445,6 +445,51 @@ DRKV_API int drkv_k_decode_attention_noalloc(const drkv_geometry* g, const void*
                                              const int32_t* d_block_table, void* out, int layer,
                                              int seq_len, int max_pages, float scale, void* stream);
 
+/* ---- rotary positions on query and key rows --------------------------------------------
+ * rope_kernel (src/machina/layer_attention.cu:32-79) for Q and K rows in the caller's memory, both in one launch, with
+ * what the reference does not have: both layouts, frequency scaling for long contexts, strides and the transpose.  (The
+ * engine's appends rotate K themselves when drkv_geometry.rotary_dim > 0, in the halves layout without scaling and with
+ * fp32 angles; a caller who rotates K here creates the engine with rotary_dim = 0.)
+ *   y0 = a (x0 cos - x1 sin), y1 = a (x1 cos + x0 sin), angle = position * f_i for pair i of rotary_dim / 2;
+ *   dims from rotary_dim on are copied.  Angles are exact to far below fp32 at every int32 position, negative ones too.
+ * Scaling of f_i = theta^(-2i / rotary_dim):
+ *   LINEAR  f_i / factor
+ *   BASE    theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta
+ *   BANDS   by the turns n = original_context * f_i / 2pi: kept for n >= high_freq_factor, f_i / factor for
+ *           n <= low_freq_factor, a linear blend of the two between
+ *   RAMP    (YaRN) f_i / factor and f_i blended by a linear ramp over the pairs from the one that makes beta_fast turns
+ *           (rounded down) to the one that makes beta_slow (rounded up); a = 0.1 ln(factor) + 1 */
+enum { DRKV_ROPE_HALVES = 0, DRKV_ROPE_PAIRS = 1 };   /* (x[i], x[i + rotary_dim/2]) or (x[2i], x[2i + 1]) */
+enum { DRKV_ROPE_NONE = 0, DRKV_ROPE_LINEAR = 1, DRKV_ROPE_BASE = 2, DRKV_ROPE_BANDS = 3, DRKV_ROPE_RAMP = 4 };
+typedef struct drkv_rope_config {
+    int32_t head_dim;          /* a multiple of 8, up to 512 */
+    int32_t rotary_dim;        /* even, 2 .. head_dim */
+    int32_t layout, dtype, scaling;
+    int32_t device;            /* CUDA device ordinal; -1 = frequencies only */
+    int32_t original_context;  /* BANDS, RAMP */
+    float low_freq_factor, high_freq_factor;   /* BANDS */
+    float beta_fast, beta_slow;                /* RAMP */
+    float attention_factor;    /* a; 0 = 1, or RAMP's own */
+    double theta, factor;
+} drkv_rope_config;
+/* Rows of one tensor, strides in elements: element (token, head, dim) is at token * token_stride + head * head_stride +
+ * dim.  src may be dst with the same strides (in place); other overlaps are refused. */
+typedef struct drkv_rope_rows {
+    const void* src;
+    void* dst;
+    int32_t heads;
+    int64_t src_token_stride, src_head_stride, dst_token_stride, dst_head_stride;
+} drkv_rope_rows;
+typedef struct drkv_rope drkv_rope;
+DRKV_API int drkv_rope_create(const drkv_rope_config* cfg, drkv_rope** out);
+DRKV_API void drkv_rope_destroy(drkv_rope* r);
+/* f_i in radians per position; returns rotary_dim / 2, writes at most cap of them. */
+DRKV_API int drkv_rope_frequencies(const drkv_rope* r, double* out, int cap);
+/* Rotates the rows of q and of k (either may be NULL, not both); d_pos[n_tokens] are device int32 positions.  inverse = 1
+ * applies the transpose, which is the gradient with respect to the rows (the rotation by the negative angle, times a). */
+DRKV_API int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, const drkv_rope_rows* q,
+                             const drkv_rope_rows* k, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
