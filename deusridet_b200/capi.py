@@ -9,7 +9,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdrkv.so")
 
 OK, ERR_INVALID, ERR_EXHAUSTED, ERR_NO_DEVICE, ERR_CUDA, ERR_STATE, ERR_CAPACITY = 0, -1, -2, -3, -4, -5, -6
-F16, BF16 = 0, 1
+F16, BF16, F16_KV_E4M3, BF16_KV_E4M3 = 0, 1, 2, 3
 
 
 class DrkvError(RuntimeError):
@@ -162,6 +162,11 @@ SIGNATURES = {
     "drkv_k_decode_scratch_bytes": (_sz, [C.POINTER(Geometry), _i]),
     "drkv_k_decode_kernel_error": (_i, [_vp, _vp]),
     "drkv_k_decode_attention_noalloc": (_i, [C.POINTER(Geometry), _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp]),
+    "drkv_page_bounds_enable": (_i, [_vp, _vp]),
+    "drkv_page_bounds": (_vp, [_vp]),
+    "drkv_page_bound_exponents": (_vp, [_vp]),
+    "drkv_select_pages": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _i, _i, _vp, _vp]),
+    "drkv_attend_selected": (_i, [_vp, _i, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _f, _vp]),
     "drkv_rope_create": (_i, [C.POINTER(RopeConfig), C.POINTER(_vp)]),
     "drkv_rope_destroy": (None, [_vp]),
     "drkv_rope_frequencies": (_i, [_vp, C.POINTER(C.c_double), _i]),

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/drkv.h"
+#include "device_guard.hpp"
 #include "kernels.hpp"
 #include "page_book.hpp"
 #include "page_store.hpp"
@@ -42,7 +43,7 @@ bool geometry_ok(const drkv_geometry& g, std::string* why) {
     if (g.num_q_heads / g.num_kv_heads > 16) return bad("GQA group larger than 16 is not supported");
     if (g.head_dim != 64 && g.head_dim != 128 && g.head_dim != 256) return bad("head_dim must be 64, 128 or 256");
     if (g.page_size <= 0 || g.page_size % 16 != 0) return bad("page_size must be a positive multiple of 16");
-    if (g.dtype != DRKV_DTYPE_F16 && g.dtype != DRKV_DTYPE_BF16) return bad("dtype must be f16 or bf16");
+    if (g.dtype < DRKV_DTYPE_F16 || g.dtype > DRKV_DTYPE_BF16_KV_E4M3) return bad("dtype must be f16 or bf16, with a pool of that type or e4m3");
     if (g.rotary_dim < 0 || g.rotary_dim > g.head_dim || g.rotary_dim % 16 != 0)
         return bad("rotary_dim must be a multiple of 16 within head_dim");
     if (g.rotary_dim > 0 && !(g.rope_theta > 0.f)) return bad("rope_theta must be positive");
@@ -56,7 +57,14 @@ void fill_inv_freq(float theta, int rot, std::vector<float>* out) {
     for (int i = 0; i < rot / 2; i++) (*out)[i] = 1.0f / powf(theta, (2.0f * (float)i) / (float)rot);
 }
 
+bool is_pool8(const drkv_geometry& g) { return g.dtype >= DRKV_DTYPE_F16_KV_E4M3; }
+// type of Q, the K and V sources and the outputs
+int io_dtype(const drkv_geometry& g) {
+    return g.dtype == DRKV_DTYPE_F16 || g.dtype == DRKV_DTYPE_F16_KV_E4M3 ? DRKV_DTYPE_F16 : DRKV_DTYPE_BF16;
+}
+
 size_t page_bytes_all_layers(const drkv_geometry& g) {
+    if (is_pool8(g)) return (size_t)g.num_layers * (size_t)Pool8Layout::make(g.num_kv_heads, g.page_size, g.head_dim, 1).block;
     return (size_t)g.num_layers * 2 * g.num_kv_heads * g.page_size * g.head_dim * 2;
 }
 
@@ -121,6 +129,16 @@ struct drkv_engine {
     std::string tmap_pf_err;
     CUtensorMap tmap_slot{};   // 4-D view, one box per 16 keys x head_dim x (K, V): the decode kernel's
     PoolLayout layout{};
+    Pool8Layout layout8{};     // 8-bit pool (pool8 only)
+    bool pool8 = false;        // K and V are stored as e4m3 with a power of two per row
+    void* d_image = nullptr;   // 8-bit pool: 16-bit image of one layer's pages, what the prefill kernel reads (tmap_pf)
+
+    // page bounds (off until drkv_page_bounds_enable)
+    struct Bounds {
+        bool on = false;
+        int8_t* d_bounds = nullptr;
+        int8_t* d_exponents = nullptr;
+    } bounds;
     int forced_chunk = 0;
     bool prefill_on_decode = false;   // chunk attention as one-token decodes even where the tensor-memory kernel could run
     int tail_mode = -1;        // tail split of the decode pass: -1 automatic (default), 0 off, n > 0: the last n chunks
@@ -210,10 +228,84 @@ static int book_err(drkv_engine* e, int rc) {
     return rc;
 }
 
+// What every launch over page bounds shares.
+static BoundsParams bounds_params(drkv_engine* e, int layer) {
+    BoundsParams p{};
+    const size_t esize = e->pool8 ? 1 : 2;
+    p.pool = static_cast<const uint8_t*>(e->pool);
+    p.plane_bytes = e->layout.kv_plane * (int64_t)esize;
+    p.block_bytes = e->pool8 ? e->layout8.block : 2 * p.plane_bytes;
+    p.layer_bytes = p.block_bytes * e->book.max_pages();
+    p.bounds = e->bounds.d_bounds;
+    p.exponents = e->bounds.d_exponents;
+    p.num_kv_heads = e->geom.num_kv_heads;
+    p.page_size = e->geom.page_size;
+    p.max_pages = e->book.max_pages();
+    p.layer = layer;
+    p.tables = e->d_tables;
+    p.table_stride = e->book.row_width();
+    p.max_rows = e->book.max_seqs();
+    return p;
+}
+// After kernels have written keys: one token of each batch entry (its position is d_pos + pos_offset) ...
+static int widen_batch(drkv_engine* e, int layer, int n, const int32_t* d_rows, const int32_t* d_pos, int pos_offset, cudaStream_t stream) {
+    if (!e->bounds.on) return DRKV_OK;
+    BoundsParams p = bounds_params(e, layer);
+    p.n_items = n;
+    p.rows = d_rows;
+    p.pos = d_pos;
+    p.pos_offset = pos_offset;
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), 1, stream));
+    return DRKV_OK;
+}
+// ... or tokens [pos_start, pos_start + m) of one sequence, in num_layers layers ...
+static int widen_range(drkv_engine* e, int layer, int num_layers, int row, int pos_start, int m, cudaStream_t stream) {
+    if (!e->bounds.on || m <= 0) return DRKV_OK;
+    BoundsParams p = bounds_params(e, layer);
+    const int P = e->geom.page_size;
+    p.n_items = (int)(((int64_t)pos_start + m - 1) / P - pos_start / P + 1);
+    p.row = row;
+    p.pos_start = pos_start;
+    p.m = m;
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), num_layers, stream));
+    return DRKV_OK;
+}
+// ... or whole pages, every layer and slot.
+static int rebuild_pages(drkv_engine* e, int page0, int n, cudaStream_t stream) {
+    if (!e->bounds.on || n <= 0) return DRKV_OK;
+    BoundsParams p = bounds_params(e, 0);
+    p.tables = nullptr;
+    p.n_items = n;
+    p.page0 = page0;
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), e->geom.num_layers, stream));
+    return DRKV_OK;
+}
+// Pages that came back from the storage tier get their bounds anew (all of a page's slots: a partly filled page's bounds
+// may be wider than its keys until its slot 0 is written again).
+static int rebuild_swapped_in(drkv_engine* e, cudaStream_t stream) {
+    if (!e->store) return DRKV_OK;
+    std::vector<int> pages;
+    e->store->take_swapped_in(&pages);
+    for (int page : pages) {
+        int rc = rebuild_pages(e, page, 1, stream);
+        if (rc != DRKV_OK) return rc;
+    }
+    return DRKV_OK;
+}
+
 static int run_cow(drkv_engine* e, const std::vector<CowJob>& jobs, cudaStream_t stream) {
+    int rc = rebuild_swapped_in(e, stream);
+    if (rc != DRKV_OK) return rc;
     for (const CowJob& j : jobs) {
-        e->cow_bytes += (int64_t)j.n_slots * e->geom.head_dim * 2 * 2 * e->geom.num_kv_heads * e->geom.num_layers;
+        e->cow_bytes += (int64_t)j.n_slots * e->geom.head_dim * 2 * (e->pool8 ? 1 : 2) * e->geom.num_kv_heads * e->geom.num_layers;
         if (!e->has_device) continue;
+        if (e->bounds.on)
+            CUDA_TRY(launch_bounds_copy(bounds_params(e, 0), e->geom.head_dim, j.src_page, j.dst_page, e->geom.num_layers, stream));
+        if (e->pool8) {
+            if (j.n_slots > 0)
+                CUDA_TRY(launch_cow_copy8(e->layout8, static_cast<uint8_t*>(e->pool), j.src_page, j.dst_page, e->geom.num_layers, stream));
+            continue;
+        }
         CowParams cp;
         cp.layout = e->layout;
         cp.pool = e->pool;
@@ -253,6 +345,8 @@ int drkv_create(const drkv_geometry* geom, const drkv_config* cfg, drkv_engine**
                        cfg->budget_bytes / 1048576.0, per_page / 1048576.0);
     }
     e->layout = PoolLayout::make(geom->num_kv_heads, geom->page_size, geom->head_dim, (int)max_pages);
+    e->pool8 = is_pool8(*geom);
+    if (e->pool8) e->layout8 = Pool8Layout::make(geom->num_kv_heads, geom->page_size, geom->head_dim, (int)max_pages);
     e->pool_bytes = per_page * (size_t)max_pages;
 
     if (cfg->device >= 0) {
@@ -307,15 +401,23 @@ int drkv_create(const drkv_geometry* geom, const drkv_config* cfg, drkv_engine**
         if (row_tokens > pool_tokens) row_tokens = pool_tokens;
         size_t need = (size_t)cfg->max_seqs * geom->num_q_heads * ((row_tokens + 255) / 256) * (geom->head_dim + 2) * 4;
         e->scratch_bytes = need < (64u << 20) ? (64u << 20) : need;
+        const size_t pieces = attend_pages_scratch_bytes(geom->num_q_heads / geom->num_kv_heads, geom->head_dim, e->num_sms);
+        if (e->scratch_bytes < pieces) e->scratch_bytes = pieces;
         if ((ce = cudaMalloc(&e->d_scratch, e->scratch_bytes)) != cudaSuccess) return fail(DRKV_ERR_CUDA, "cudaMalloc(scratch)", ce);
         const char* terr = nullptr;
+        if (e->pool8) {
+            const size_t image = 2 * (size_t)e->layout8.plane * 2 * (size_t)max_pages;
+            if ((ce = cudaMalloc(&e->d_image, image)) != cudaSuccess) return fail(DRKV_ERR_CUDA, "cudaMalloc(image)", ce);
+            // pages never written hold what cudaMalloc left; the prefill kernel reads whole 16-key groups of listed pages only
+            if ((ce = cudaMemset(e->d_image, 0, image)) != cudaSuccess) return fail(DRKV_ERR_CUDA, "cudaMemset(image)", ce);
+        }
         {
             const char* perr = nullptr;
-            e->has_tmap_pf = make_pool_kv16_tensor_map(&e->tmap_pf, e->pool, geom->num_layers, (int)max_pages,
+            e->has_tmap_pf = make_pool_kv16_tensor_map(&e->tmap_pf, e->pool8 ? e->d_image : e->pool, e->pool8 ? 1 : geom->num_layers, (int)max_pages,
                                                        geom->num_kv_heads, geom->page_size, geom->head_dim, &perr);
             if (!e->has_tmap_pf) e->tmap_pf_err = perr ? perr : "tensor map";   // prefill then runs on the decode kernel
         }
-        if (!make_pool_slot_tensor_map(&e->tmap_slot, e->pool, geom->num_layers, (int)max_pages, geom->num_kv_heads,
+        if (!e->pool8 && !make_pool_slot_tensor_map(&e->tmap_slot, e->pool, geom->num_layers, (int)max_pages, geom->num_kv_heads,
                                        geom->page_size, geom->head_dim, &terr)) {
             set_err(DRKV_ERR_CUDA, "%s", terr ? terr : "tensor map");
             drkv_destroy(e);
@@ -344,6 +446,9 @@ void drkv_destroy(drkv_engine* e) {
         cudaFree(e->d_error);
         cudaFree(e->d_scratch);
         cudaFree(e->d_plan);
+        cudaFree(e->d_image);
+        cudaFree(e->bounds.d_bounds);
+        cudaFree(e->bounds.d_exponents);
         cudaFree(e->scorer.d_scores);
         cudaFree(e->scorer.d_fresh);
         cudaFree(e->scorer.d_tile_lse);
@@ -409,9 +514,11 @@ int drkv_pool_page_size(const drkv_engine* e) { return e ? e->book.page_size() :
 void* drkv_pool_ptr(const drkv_engine* e) { return e ? e->pool : nullptr; }
 size_t drkv_pool_total_bytes(const drkv_engine* e) { return e ? e->pool_bytes : 0; }
 size_t drkv_pool_k_offset(const drkv_engine* e, int layer, int page) {
+    if (e && e->pool8) return (size_t)e->layout8.block_of(layer, page);
     return e ? (size_t)e->layout.row(layer, page, 0, 0, 0) * 2 : 0;  // block_pool.cpp:89-91
 }
 size_t drkv_pool_v_offset(const drkv_engine* e, int layer, int page) {
+    if (e && e->pool8) return (size_t)(e->layout8.block_of(layer, page) + e->layout8.plane);
     return e ? (size_t)e->layout.row(layer, page, 1, 0, 0) * 2 : 0;  // block_pool.cpp:93-95
 }
 
@@ -687,6 +794,7 @@ int drkv_set_tail_split(drkv_engine* e, int mode) {
 
 int drkv_set_prefill_on_decode_kernel(drkv_engine* e, int on) {
     NEED(e);
+    if (on && e->pool8) return set_err(DRKV_ERR_INVALID, "prefill on the decode kernel: not with an 8-bit pool");
     e->prefill_on_decode = on != 0;
     return DRKV_OK;
 }
@@ -736,6 +844,27 @@ static AppendParams append_params(drkv_engine* e, int layer) {
     return p;
 }
 
+static int append8(drkv_engine* e, int layer, int n, const int32_t* d_rows, const int32_t* d_pos, int row, int pos_start,
+                   const void* k_src, const void* v_src, cudaStream_t stream) {
+    Append8Params p{};
+    p.layout = e->layout8;
+    p.pool = static_cast<uint8_t*>(e->pool);
+    p.tables = e->d_tables;
+    p.table_stride = e->book.row_width();
+    p.max_rows = e->book.max_seqs();
+    p.rows = d_rows;
+    p.pos = d_pos;
+    p.row = row;
+    p.pos_start = pos_start;
+    p.layer = layer;
+    p.rotary_dim = e->geom.rotary_dim;
+    p.inv_freq = e->d_inv_freq;
+    p.k_src = k_src;
+    p.v_src = v_src;
+    CUDA_TRY(launch_append8(p, n, io_dtype(e->geom), stream));
+    return DRKV_OK;
+}
+
 int drkv_append_rope(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_pos,
                      const void* k_src, const void* v_src, void* stream) {
     NEED(e);
@@ -743,13 +872,18 @@ int drkv_append_rope(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows
     if (layer < 0 || layer >= e->geom.num_layers || n_seq < 0 || !d_rows || !d_pos || !k_src || !v_src)
         return set_err(DRKV_ERR_INVALID, "append_rope: bad argument");
     note_stream(e, (cudaStream_t)stream);
+    if (e->pool8) {
+        DeviceGuard dev(e->device);
+        int rc = append8(e, layer, n_seq, d_rows, d_pos, 0, 0, k_src, v_src, (cudaStream_t)stream);
+        return rc == DRKV_OK ? widen_batch(e, layer, n_seq, d_rows, d_pos, 0, (cudaStream_t)stream) : rc;
+    }
     AppendParams p = append_params(e, layer);
     p.rows = d_rows;
     p.pos = d_pos;
     p.k_src = k_src;
     p.v_src = v_src;
     CUDA_TRY(launch_append_rope(p, n_seq, e->geom.dtype, (cudaStream_t)stream));
-    return DRKV_OK;
+    return widen_batch(e, layer, n_seq, d_rows, d_pos, 0, (cudaStream_t)stream);
 }
 
 int drkv_append_rope_chunk(drkv_engine* e, int layer, int seq, int pos_start, int m, const void* k_src,
@@ -760,6 +894,14 @@ int drkv_append_rope_chunk(drkv_engine* e, int layer, int seq, int pos_start, in
         seq >= e->book.max_seqs())
         return set_err(DRKV_ERR_INVALID, "append_rope_chunk: bad argument");
     note_stream(e, (cudaStream_t)stream);
+    if (e->pool8 || e->bounds.on) {
+        if (m > INT32_MAX - pos_start) return set_err(DRKV_ERR_INVALID, "append_rope_chunk: positions beyond 2^31");
+    }
+    if (e->pool8) {
+        DeviceGuard dev(e->device);
+        int rc = append8(e, layer, m, nullptr, nullptr, seq, pos_start, k_src, v_src, (cudaStream_t)stream);
+        return rc == DRKV_OK ? widen_range(e, layer, 1, seq, pos_start, m, (cudaStream_t)stream) : rc;
+    }
     AppendParams p = append_params(e, layer);
     p.rows = nullptr;
     p.pos = nullptr;
@@ -768,13 +910,29 @@ int drkv_append_rope_chunk(drkv_engine* e, int layer, int seq, int pos_start, in
     p.k_src = k_src;
     p.v_src = v_src;
     CUDA_TRY(launch_append_rope(p, m, e->geom.dtype, (cudaStream_t)stream));
-    return DRKV_OK;
+    return widen_range(e, layer, 1, seq, pos_start, m, (cudaStream_t)stream);
 }
 
 static int seq_flat_copy(drkv_engine* e, int seq, int start_token, int num_tokens, void* flat, bool to_flat,
                          void* stream) {
     if (seq < 0 || seq >= e->book.max_seqs() || start_token < 0 || num_tokens < 0 || !flat)
         return set_err(DRKV_ERR_INVALID, "extract/inject: bad argument");
+    if (num_tokens > INT32_MAX - start_token) return set_err(DRKV_ERR_INVALID, "extract/inject: positions beyond 2^31");
+    if (e->pool8) {
+        DeviceGuard dev(e->device);
+        note_stream(e, (cudaStream_t)stream);
+        Flat8Params f{};
+        f.layout = e->layout8;
+        f.pool = static_cast<uint8_t*>(e->pool);
+        f.flat = flat;
+        f.table = e->d_tables + (size_t)seq * e->book.row_width();
+        f.table_stride = e->book.row_width();
+        f.start_token = start_token;
+        f.num_tokens = num_tokens;
+        f.num_layers = e->geom.num_layers;
+        CUDA_TRY(launch_flat_copy8(f, to_flat, io_dtype(e->geom), (cudaStream_t)stream));
+        return to_flat ? DRKV_OK : widen_range(e, 0, e->geom.num_layers, seq, start_token, num_tokens, (cudaStream_t)stream);
+    }
     FlatCopyParams p{};
     p.layout = e->layout;
     p.pool = e->pool;
@@ -785,7 +943,7 @@ static int seq_flat_copy(drkv_engine* e, int seq, int start_token, int num_token
     p.num_tokens = num_tokens;
     p.num_layers = e->geom.num_layers;
     CUDA_TRY(launch_flat_paged_copy(p, to_flat, e->num_sms, (cudaStream_t)stream));
-    return DRKV_OK;
+    return to_flat ? DRKV_OK : widen_range(e, 0, e->geom.num_layers, seq, start_token, num_tokens, (cudaStream_t)stream);
 }
 
 int drkv_seq_extract(drkv_engine* e, int seq, int start_token, int num_tokens, void* dst, void* stream) {
@@ -950,6 +1108,57 @@ static int decode_common(drkv_engine* e, int layer, int n_seq, const int32_t* d_
     return DRKV_OK;
 }
 
+// Decode attention over the 8-bit pool, and over listed pages of either pool (attend_pages.cu).
+static int attend_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
+                        const int32_t* d_list, int list_len, const void* q, void* out, float scale, cudaStream_t stream) {
+    const drkv_geometry& g = e->geom;
+    DeviceGuard dev(e->device);
+    note_stream(e, stream);
+    const int64_t row_tokens = (int64_t)e->book.row_width() * g.page_size;
+    if (max_kv_len > row_tokens) max_kv_len = (int)row_tokens;
+    const BoundsParams strides = bounds_params(e, layer);
+    AttendPagesParams p{};
+    p.pool = strides.pool + (int64_t)layer * strides.layer_bytes;
+    p.block_bytes = strides.block_bytes;
+    p.plane_bytes = strides.plane_bytes;
+    p.exp_plane_bytes = e->layout8.exp_plane;
+    p.tables = e->d_tables;
+    p.table_stride = e->book.row_width();
+    p.max_rows = e->book.max_seqs();
+    p.max_pages = e->book.max_pages();
+    p.max_kv_len = max_kv_len;
+    p.list_len = list_len;
+    p.num_kv_heads = g.num_kv_heads;
+    p.group = g.num_q_heads / g.num_kv_heads;
+    p.page_size = g.page_size;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.scratch = e->d_scratch;
+    p.error_word = e->d_error;
+    // the kernel counts 16-key groups of a launch in 32 bits
+    int64_t groups = ((int64_t)max_kv_len + 15) / 16;
+    if (d_list && (int64_t)list_len * (g.page_size / 16) < groups) groups = (int64_t)list_len * (g.page_size / 16);
+    const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxDecodeSeqs;
+    if (cap < 1) return set_err(DRKV_ERR_CAPACITY, "attend: %d keys of %d KV heads are more than one launch takes", max_kv_len, g.num_kv_heads);
+    const int step = cap < kMaxDecodeSeqs ? (int)cap : kMaxDecodeSeqs;
+    const size_t row_bytes = (size_t)g.num_q_heads * g.head_dim * 2;
+    for (int s0 = 0; s0 < n_seq; s0 += step) {
+        p.n_seq = n_seq - s0 < step ? n_seq - s0 : step;
+        p.rows = d_rows + s0;
+        p.kv_len = d_kv_len + s0;
+        p.list = d_list ? d_list + (int64_t)s0 * g.num_kv_heads * list_len : nullptr;
+        p.q = (const char*)q + s0 * row_bytes;
+        p.out = (char*)out + s0 * row_bytes;
+        const bool timed = e->timing && e->tev_used + 2 <= e->tev.size();
+        if (timed) CUDA_TRY(cudaEventRecord(e->tev[e->tev_used], stream));
+        CUDA_TRY(launch_attend_pages(p, e->pool8, g.head_dim, io_dtype(g), e->num_sms, stream));
+        if (timed) {
+            CUDA_TRY(cudaEventRecord(e->tev[e->tev_used + 1], stream));
+            e->tev_used += 2;
+        }
+    }
+    return DRKV_OK;
+}
+
 int drkv_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
                        int max_kv_len, const void* q, void* out, float scale, void* stream) {
     NEED(e);
@@ -957,6 +1166,8 @@ int drkv_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_t* d_ro
     if (layer < 0 || layer >= e->geom.num_layers || n_seq < 0 || !d_rows || !d_kv_len || !q || !out || max_kv_len < 0)
         return set_err(DRKV_ERR_INVALID, "attend_decode: bad argument");
     if (n_seq == 0 || max_kv_len == 0) return DRKV_OK;
+    if (e->pool8)
+        return attend_pages(e, layer, n_seq, d_rows, d_kv_len, max_kv_len, nullptr, 0, q, out, scale, (cudaStream_t)stream);
     // one launch takes up to kMaxDecodeSeqs sequences; larger batches go in slices
     const size_t row_bytes = (size_t)e->geom.num_q_heads * e->geom.head_dim * 2;
     for (int s0 = 0; s0 < n_seq; s0 += kMaxDecodeSeqs) {
@@ -969,6 +1180,15 @@ int drkv_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_t* d_ro
     return DRKV_OK;
 }
 
+// The decode step over the 8-bit pool: the append is a launch of its own (positions d_kv_len - 1).
+static int append_attend8(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
+                          const void* k_src, const void* v_src, const void* q, void* out, float scale, cudaStream_t stream) {
+    DeviceGuard dev(e->device);
+    int rc = append8(e, layer, n_seq, d_rows, d_kv_len, 0, -1, k_src, v_src, stream);
+    if (rc == DRKV_OK) rc = widen_batch(e, layer, n_seq, d_rows, d_kv_len, -1, stream);
+    return rc == DRKV_OK ? attend_pages(e, layer, n_seq, d_rows, d_kv_len, max_kv_len, nullptr, 0, q, out, scale, stream) : rc;
+}
+
 int drkv_append_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
                               int max_kv_len, const void* k_src, const void* v_src, const void* q, void* out, float scale,
                               void* stream) {
@@ -978,6 +1198,7 @@ int drkv_append_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_
         max_kv_len < 0)
         return set_err(DRKV_ERR_INVALID, "append_attend_decode: bad argument");
     if (n_seq == 0 || max_kv_len == 0) return DRKV_OK;
+    if (e->pool8) return append_attend8(e, layer, n_seq, d_rows, d_kv_len, max_kv_len, k_src, v_src, q, out, scale, (cudaStream_t)stream);
     // every head dim appends inside the decode kernel (at head dim 256, whose ring holds K and V of a group in separate
     // entries, the K row is staged and the V row taken from its source)
     const size_t q_bytes = (size_t)e->geom.num_q_heads * e->geom.head_dim * 2;
@@ -990,7 +1211,7 @@ int drkv_append_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_
                                (const char*)k_src + s0 * kv_bytes, (const char*)v_src + s0 * kv_bytes);
         if (rc != DRKV_OK) return rc;
     }
-    return DRKV_OK;
+    return widen_batch(e, layer, n_seq, d_rows, d_kv_len, -1, (cudaStream_t)stream);
 }
 
 int drkv_plan_decode(drkv_engine* e, int n_seq, const int32_t* seqs, const int32_t* kv_len, void* stream_) {
@@ -1019,7 +1240,7 @@ int drkv_plan_decode(drkv_engine* e, int n_seq, const int32_t* seqs, const int32
         max_kv = kv_len[i] > max_kv ? kv_len[i] : max_kv;
         keys_seq += kv_len[i];
     }
-    for (int i = 0; i < n_seq && per_block >= 2;) {
+    for (int i = 0; i < n_seq && per_block >= 2 && !e->pool8;) {   // an 8-bit pool's planned pass is the per-sequence one
         const std::vector<int32_t>& lead = e->book.seq(seqs[i])->table;
         int shared = kv_len[i], j = i + 1;
         for (; j < n_seq; j++) {
@@ -1171,6 +1392,8 @@ int drkv_attend_decode_planned(drkv_engine* e, int layer, const void* q, void* o
     const drkv_engine::Plan& pl = e->plan;
     if (!pl.valid) return set_err(DRKV_ERR_INVALID, "attend_decode_planned: no decode plan");
     if (pl.n_seq == 0 || pl.max_chunks == 0) return DRKV_OK;
+    if (e->pool8)
+        return attend_pages(e, layer, pl.n_seq, pl.rows, pl.kv_len, pl.max_chunks * pl.chunk, nullptr, 0, q, out, scale, (cudaStream_t)stream);
     return decode_common(e, layer, pl.n_seq, pl.rows, pl.kv_len, 0, 0, 0, pl.max_chunks * pl.chunk, q, out, nullptr,
                          scale, (cudaStream_t)stream, &pl);
 }
@@ -1184,8 +1407,12 @@ int drkv_append_attend_decode_planned(drkv_engine* e, int layer, const void* k_s
     const drkv_engine::Plan& pl = e->plan;
     if (!pl.valid) return set_err(DRKV_ERR_INVALID, "append_attend_decode_planned: no decode plan");
     if (pl.n_seq == 0 || pl.max_chunks == 0) return DRKV_OK;
-    return decode_common(e, layer, pl.n_seq, pl.rows, pl.kv_len, 0, 0, 0, pl.max_chunks * pl.chunk, q, out, nullptr,
-                         scale, (cudaStream_t)stream, &pl, nullptr, 0, k_src, v_src);
+    if (e->pool8)
+        return append_attend8(e, layer, pl.n_seq, pl.rows, pl.kv_len, pl.max_chunks * pl.chunk, k_src, v_src, q, out, scale,
+                              (cudaStream_t)stream);
+    int rc = decode_common(e, layer, pl.n_seq, pl.rows, pl.kv_len, 0, 0, 0, pl.max_chunks * pl.chunk, q, out, nullptr,
+                           scale, (cudaStream_t)stream, &pl, nullptr, 0, k_src, v_src);
+    return rc == DRKV_OK ? widen_batch(e, layer, pl.n_seq, pl.rows, pl.kv_len, -1, (cudaStream_t)stream) : rc;
 }
 
 // ---- storage tier --------------------------------------------------------------------------
@@ -1195,7 +1422,8 @@ int drkv_tier_enable(drkv_engine* e, const char* dir) {
     LOCK(e);
     std::unique_ptr<PageStore> st(new PageStore());
     std::string err;
-    const size_t page_bytes = (size_t)2 * e->geom.num_kv_heads * e->geom.page_size * e->geom.head_dim * 2;
+    const size_t page_bytes = e->pool8 ? (size_t)e->layout8.block
+                                       : (size_t)2 * e->geom.num_kv_heads * e->geom.page_size * e->geom.head_dim * 2;
     if (!st->init(dir, e->pool, e->geom.num_layers, page_bytes * (size_t)e->book.max_pages(), page_bytes, &err))
         return set_err(DRKV_ERR_STATE, "%s", err.c_str());
     st->set_order_stream(e->last_stream);
@@ -1259,7 +1487,7 @@ int drkv_tier_file_to_page(drkv_engine* e, const char* path, int page) {
     if (!e->store) return set_err(DRKV_ERR_STATE, "tier_file_to_page: no storage tier");
     if (!path || page < 0 || page >= e->book.max_pages()) return set_err(DRKV_ERR_INVALID, "tier_file_to_page: bad argument");
     if (!e->store->file_to_page(path, page)) return set_err(DRKV_ERR_STATE, "tier_file_to_page: read or copy failed (%s)", path);
-    return DRKV_OK;
+    return rebuild_pages(e, page, 1, e->last_stream);
 }
 
 int drkv_tier_drain(drkv_engine* e) {
@@ -1304,6 +1532,7 @@ int drkv_scorer_enable(drkv_engine* e, float decay) {
     NEED(e);
     LOCK(e);
     drkv_engine::Scorer& sc = e->scorer;
+    if (decay >= 0.f && e->pool8) return set_err(DRKV_ERR_INVALID, "scorer_enable: attention over an 8-bit pool yields no page masses");
     if (!(decay >= 0.f)) {                               // negative: detach; eviction is oldest-first again
         sc.on = false;
         e->book.attach_scores(nullptr);
@@ -1388,6 +1617,7 @@ int drkv_attend_partial(drkv_engine* e, int layer, int seq, int kv_begin, int kv
     NEED_DEVICE(e);
     if (layer < 0 || layer >= e->geom.num_layers || seq < 0 || seq >= e->book.max_seqs() || kv_begin < 0 || !q || !part)
         return set_err(DRKV_ERR_INVALID, "attend_partial: bad argument");
+    if (e->pool8) return set_err(DRKV_ERR_INVALID, "attend_partial: not with an 8-bit pool");
     int span = kv_end - (kv_begin / 16) * 16;
     if (span < 1) span = 1;   // an empty range still has to produce the (-1e20, 0, 0) partial
     return decode_common(e, layer, 1, nullptr, nullptr, seq, kv_begin, kv_end, span, q, nullptr, part, scale,
@@ -1410,6 +1640,7 @@ int drkv_exchange_create(drkv_engine* e, int world, int rank, uint8_t* handle_ou
     NEED_DEVICE(e);
     if (world < 1 || world > kMaxExchangeRanks || rank < 0 || rank >= world || !handle_out)
         return set_err(DRKV_ERR_INVALID, "exchange_create: bad argument (at most %d ranks)", kMaxExchangeRanks);
+    if (e->pool8) return set_err(DRKV_ERR_INVALID, "exchange_create: not with an 8-bit pool");
     static_assert(sizeof(cudaIpcMemHandle_t) == DRKV_IPC_HANDLE_BYTES, "IPC handle size");
     LOCK(e);
     CUDA_TRY(cudaSetDevice(e->device));
@@ -1518,6 +1749,7 @@ static int attend_exchange(drkv_engine* e, int layer, int seq, int kv_begin, int
     p.parity = (int)(p.seq_no & 1u);
     p.wait_ns = x.wait_ns;
     p.error_word = e->d_error;
+    const bool appends = k_src != nullptr;
     if (k_src != nullptr && kv_end <= kv_begin) {
         // nothing of this rank's range to attend: the token goes through the append kernel
         if (kv_end < 1) return set_err(DRKV_ERR_INVALID, "append_attend_exchange: no position to append at");
@@ -1533,15 +1765,16 @@ static int attend_exchange(drkv_engine* e, int layer, int seq, int kv_begin, int
         k_src = v_src = nullptr;
     }
     // the merge kernel's CTA of head h exchanges that head with the peers and writes the final output
-    return decode_common(e, layer, 1, nullptr, nullptr, seq, kv_begin, kv_end, span, q, out, nullptr, scale,
-                         (cudaStream_t)stream, nullptr, &p, 0, k_src, v_src);
+    int rc = decode_common(e, layer, 1, nullptr, nullptr, seq, kv_begin, kv_end, span, q, out, nullptr, scale,
+                           (cudaStream_t)stream, nullptr, &p, 0, k_src, v_src);
+    return rc == DRKV_OK && appends ? widen_range(e, layer, 1, seq, kv_end - 1, 1, (cudaStream_t)stream) : rc;
 }
 
 int drkv_combine_partials(drkv_engine* e, int n_parts, const float* parts, void* out, void* stream) {
     NEED(e);
     NEED_DEVICE(e);
     if (n_parts < 0 || !parts || !out) return set_err(DRKV_ERR_INVALID, "combine_partials: bad argument");
-    CUDA_TRY(launch_combine_external(n_parts, parts, e->geom.num_q_heads, e->geom.head_dim, out, e->geom.dtype,
+    CUDA_TRY(launch_combine_external(n_parts, parts, e->geom.num_q_heads, e->geom.head_dim, out, io_dtype(e->geom),
                                      (cudaStream_t)stream));
     return DRKV_OK;
 }
@@ -1579,6 +1812,8 @@ int drkv_attend_prefill_batch(drkv_engine* e, int layer, int n_seq, const int32_
     for (int i = 0; i < n_seq; i++)
         if (seqs[i] < 0 || seqs[i] >= e->book.max_seqs() || pos_start[i] < 0 || m[i] < 0 || (m[i] > 0 && (!q[i] || !out[i])))
             return set_err(DRKV_ERR_INVALID, "attend_prefill: bad sequence entry %d", i);
+    if (e->pool8 && !e->has_tmap_pf) return set_err(DRKV_ERR_CAPACITY, "attend_prefill: one layer of the pool is more than a TMA descriptor addresses");
+    DeviceGuard dev(e->device);
     if (!e->has_tmap_pf || e->prefill_on_decode) {
         // no 16-key view of this pool for the tensor-memory kernel (a pool beyond what one TMA descriptor addresses),
         // or the caller asked for it: the chunk runs on the split-KV decode kernel, a batch of one-token decodes over
@@ -1604,6 +1839,25 @@ int drkv_attend_prefill_batch(drkv_engine* e, int layer, int n_seq, const int32_
             p.out[i] = out[s0 + i];
         }
         p.layer = layer;
+        if (e->pool8) {
+            // the sequences' pages of this layer as 16 bits, then the kernel as it stands over that image: a 2 048-token
+            // chunk reuses a key some thousand times, so the copy is a few percent of it
+            note_stream(e, (cudaStream_t)stream);
+            Expand8Params x{};
+            x.layout = e->layout8;
+            x.pool = static_cast<const uint8_t*>(e->pool);
+            x.image = e->d_image;
+            x.tables = e->d_tables;
+            x.table_stride = e->book.row_width();
+            x.layer = layer;
+            x.n_seq = p.n_seq;
+            for (int i = 0; i < p.n_seq; i++) {
+                x.row[i] = p.row[i];
+                x.n_tokens[i] = p.m[i] == 0 ? 0 : p.m[i] > INT32_MAX - p.pos_start[i] ? INT32_MAX : p.pos_start[i] + p.m[i];
+            }
+            CUDA_TRY(launch_expand8(x, io_dtype(g), (cudaStream_t)stream));
+            p.layer = 0;
+        }
         p.max_pages = e->book.max_pages();
         p.num_q_heads = g.num_q_heads;
         p.num_kv_heads = g.num_kv_heads;
@@ -1611,10 +1865,101 @@ int drkv_attend_prefill_batch(drkv_engine* e, int layer, int n_seq, const int32_
         p.page_size = g.page_size;
         p.scale_log2 = scale * 1.4426950408889634f;
         p.error_word = e->d_error;
-        CUDA_TRY(launch_attend_prefill(e->tmap_pf, p, g.head_dim, g.dtype, e->num_sms, e->d_scratch, e->scratch_bytes,
+        CUDA_TRY(launch_attend_prefill(e->tmap_pf, p, g.head_dim, io_dtype(g), e->num_sms, e->d_scratch, e->scratch_bytes,
                                        (cudaStream_t)stream));
     }
     return DRKV_OK;
+}
+
+// ---- page bounds and sparse attention -------------------------------------------------------
+int drkv_page_bounds_enable(drkv_engine* e, void* stream) {
+    NEED(e);
+    NEED_DEVICE(e);
+    LOCK(e);
+    DeviceGuard dev(e->device);
+    const drkv_geometry& g = e->geom;
+    const size_t n = (size_t)g.num_layers * e->book.max_pages() * g.num_kv_heads;
+    if (e->bounds.d_bounds == nullptr) {
+        int8_t *b = nullptr, *x = nullptr;
+        cudaError_t ce = cudaMalloc(&b, n * 2 * g.head_dim);
+        if (ce == cudaSuccess) ce = cudaMalloc(&x, n);
+        if (ce != cudaSuccess) {
+            cudaFree(b);
+            return set_err(DRKV_ERR_CUDA, "page_bounds_enable: %s", cudaGetErrorString(ce));
+        }
+        e->bounds.d_bounds = b;
+        e->bounds.d_exponents = x;
+    }
+    note_stream(e, (cudaStream_t)stream);
+    e->bounds.on = true;
+    if (e->store) {
+        std::vector<int> pages;
+        e->store->take_swapped_in(&pages);       // every page is about to be done
+    }
+    return rebuild_pages(e, 0, e->book.max_pages(), (cudaStream_t)stream);
+}
+
+const int8_t* drkv_page_bounds(const drkv_engine* e) { return e ? e->bounds.d_bounds : nullptr; }
+const int8_t* drkv_page_bound_exponents(const drkv_engine* e) { return e ? e->bounds.d_exponents : nullptr; }
+
+int drkv_select_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
+                      const void* q, int top_pages, int first_pages, int last_pages, int32_t* d_sel, void* stream) {
+    NEED(e);
+    NEED_DEVICE(e);
+    const drkv_geometry& g = e->geom;
+    if (layer < 0 || layer >= g.num_layers || n_seq < 0 || max_kv_len < 0 || !d_rows || !d_kv_len || !q || !d_sel)
+        return set_err(DRKV_ERR_INVALID, "select_pages: bad argument");
+    if (top_pages < 1 || first_pages < 0 || last_pages < 0 || (int64_t)first_pages + last_pages > top_pages)
+        return set_err(DRKV_ERR_INVALID, "select_pages: top_pages must be positive and hold first_pages + last_pages");
+    if (!e->bounds.on) return set_err(DRKV_ERR_STATE, "select_pages: page bounds are not enabled");
+    if (n_seq == 0) return DRKV_OK;
+    DeviceGuard dev(e->device);
+    note_stream(e, (cudaStream_t)stream);
+    const int64_t row_tokens = (int64_t)e->book.row_width() * g.page_size;
+    if (max_kv_len > row_tokens) max_kv_len = (int)row_tokens;
+    SelectParams p{};
+    p.bounds = e->bounds.d_bounds;
+    p.exponents = e->bounds.d_exponents;
+    p.tables = e->d_tables;
+    p.table_stride = e->book.row_width();
+    p.max_rows = e->book.max_seqs();
+    p.max_pages = e->book.max_pages();
+    p.layer = layer;
+    p.max_kv_len = max_kv_len;
+    p.num_kv_heads = g.num_kv_heads;
+    p.group = g.num_q_heads / g.num_kv_heads;
+    p.page_size = g.page_size;
+    p.top_pages = top_pages;
+    p.first_pages = first_pages;
+    p.last_pages = last_pages;
+    p.keys = reinterpret_cast<uint32_t*>(e->d_scratch);
+    p.key_stride = (int)(((int64_t)max_kv_len + g.page_size - 1) / g.page_size);
+    p.error_word = e->d_error;
+    const size_t per_seq = (size_t)g.num_kv_heads * (p.key_stride > 0 ? p.key_stride : 1) * 4;
+    if (per_seq > e->scratch_bytes) return set_err(DRKV_ERR_CAPACITY, "select_pages: the scores of %d pages exceed the scratch", p.key_stride);
+    const size_t fit = e->scratch_bytes / per_seq;
+    const int step = fit < (size_t)kMaxDecodeSeqs ? (int)fit : kMaxDecodeSeqs;
+    const size_t row_bytes = (size_t)g.num_q_heads * g.head_dim * 2;
+    for (int s0 = 0; s0 < n_seq; s0 += step) {
+        p.n_seq = n_seq - s0 < step ? n_seq - s0 : step;
+        p.rows = d_rows + s0;
+        p.kv_len = d_kv_len + s0;
+        p.q = (const char*)q + s0 * row_bytes;
+        p.sel = d_sel + (int64_t)s0 * g.num_kv_heads * top_pages;
+        CUDA_TRY(launch_select_pages(p, g.head_dim, io_dtype(g), e->num_sms, (cudaStream_t)stream));
+    }
+    return DRKV_OK;
+}
+
+int drkv_attend_selected(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
+                         const int32_t* d_sel, int top_pages, const void* q, void* out, float scale, void* stream) {
+    NEED(e);
+    NEED_DEVICE(e);
+    if (layer < 0 || layer >= e->geom.num_layers || n_seq < 0 || max_kv_len < 0 || top_pages < 1 || !d_rows || !d_kv_len ||
+        !d_sel || !q || !out)
+        return set_err(DRKV_ERR_INVALID, "attend_selected: bad argument");
+    if (n_seq == 0 || max_kv_len == 0) return DRKV_OK;
+    return attend_pages(e, layer, n_seq, d_rows, d_kv_len, max_kv_len, d_sel, top_pages, q, out, scale, (cudaStream_t)stream);
 }
 
 int drkv_attend_prefill_chunk(drkv_engine* e, int layer, int seq, int pos_start, int m, const void* q, void* out,

@@ -146,6 +146,100 @@ cudaError_t launch_importance_update(float* scores, float* fresh, int64_t n, flo
 cudaError_t launch_importance_add(float* scores, const float* new_scores, int n, float decay, cudaStream_t stream);
 
 
+// ---- the 8-bit pool (cache8.cu) ----
+struct Append8Params {
+    Pool8Layout layout;
+    uint8_t* pool;
+    const int32_t* tables;   // [rows][table_stride]
+    int table_stride, max_rows;
+    const int32_t* rows;     // per token table row and position (+ pos_start), or nullptr: one sequence, row `row` from pos_start
+    const int32_t* pos;
+    int row, pos_start;
+    int layer;
+    int rotary_dim;
+    const float* inv_freq;
+    const void* k_src;
+    const void* v_src;
+};
+cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, cudaStream_t stream);
+
+struct Flat8Params {
+    Pool8Layout layout;
+    uint8_t* pool;
+    void* flat;              // [layer][K|V][token][kv_head][dim], 16 bits an element
+    const int32_t* table;
+    int table_stride, start_token, num_tokens, num_layers;
+};
+cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, cudaStream_t stream);
+
+// Pages of up to kMaxPrefillSeqs sequences expanded into a 16-bit image of one layer with the same page ids.
+struct Expand8Params {
+    Pool8Layout layout;
+    const uint8_t* pool;
+    void* image;
+    const int32_t* tables;
+    int table_stride, layer, n_seq;
+    int row[kMaxPrefillSeqs], n_tokens[kMaxPrefillSeqs];
+};
+cudaError_t launch_expand8(const Expand8Params& p, int dtype, cudaStream_t stream);
+cudaError_t launch_cow_copy8(const Pool8Layout& layout, uint8_t* pool, int src_page, int dst_page, int num_layers, cudaStream_t stream);
+
+// ---- decode attention over the 8-bit pool, and over listed pages of either pool (attend_pages.cu) ----
+struct AttendPagesParams {
+    const uint8_t* pool;      // the layer's first block
+    int64_t block_bytes, plane_bytes, exp_plane_bytes;
+    const int32_t* tables;
+    int table_stride, max_rows, max_pages;
+    const int32_t* rows;      // [n_seq]
+    const int32_t* kv_len;    // [n_seq]
+    int max_kv_len;
+    const int32_t* list;      // [n_seq][Hkv][list_len] logical pages, nullptr: every page
+    int list_len;
+    int n_seq, num_kv_heads, group, page_size;
+    const void* q;            // [n_seq][Hq][D]
+    void* out;
+    float scale_log2;         // scale * log2(e)
+    float* scratch;           // partials and the work split, attend_pages_scratch_bytes
+    int* error_word;
+};
+size_t attend_pages_scratch_bytes(int group, int head_dim, int num_sms);
+cudaError_t launch_attend_pages(const AttendPagesParams& p, bool pool8, int head_dim, int dtype, int num_sms, cudaStream_t stream);
+
+// ---- page bounds and selection (page_bounds.cu) ----
+struct BoundsParams {
+    const uint8_t* pool;
+    int64_t layer_bytes, block_bytes, plane_bytes;
+    int8_t* bounds;           // [layer][page][Hkv][max: D, min: D]
+    int8_t* exponents;        // [layer][page][Hkv]
+    int num_kv_heads, page_size, max_pages, layer;
+    const int32_t* tables;
+    int table_stride, max_rows;
+    int n_items;              // batch entries, pages of the range, or pages (see bounds_kernel)
+    const int32_t* rows;      // batch: table row and position (+ pos_offset) of every entry
+    const int32_t* pos;
+    int pos_offset;
+    int row, pos_start, m;    // range of one sequence (tables != nullptr, rows == nullptr)
+    int page0;                // pages (tables == nullptr)
+};
+cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, cudaStream_t stream);
+cudaError_t launch_bounds_copy(const BoundsParams& p, int head_dim, int src_page, int dst_page, int num_layers, cudaStream_t stream);
+struct SelectParams {
+    const int8_t* bounds;
+    const int8_t* exponents;
+    const int32_t* tables;
+    int table_stride, max_rows, max_pages, layer;
+    const int32_t* rows;      // [n_seq]
+    const int32_t* kv_len;    // [n_seq]
+    int max_kv_len, n_seq, num_kv_heads, group, page_size;
+    const void* q;            // [n_seq][Hq][D]
+    int top_pages, first_pages, last_pages;
+    uint32_t* keys;           // [n_seq][Hkv][key_stride] workspace
+    int key_stride;
+    int32_t* sel;             // [n_seq][Hkv][top_pages]
+    int* error_word;
+};
+cudaError_t launch_select_pages(const SelectParams& p, int head_dim, int dtype, int num_sms, cudaStream_t stream);
+
 cudaError_t launch_append_rope(const AppendParams& p, int n_tokens, int dtype, cudaStream_t stream);
 cudaError_t launch_cow_copy(const CowParams& p, int num_layers, cudaStream_t stream);
 cudaError_t launch_flat_paged_copy(const FlatCopyParams& p, bool to_flat, int num_sms, cudaStream_t stream);

@@ -33,6 +33,55 @@ struct PoolLayout {
     }
 };
 
+// The 8-bit pool, in bytes.  A (layer, page) block: K rows, V rows (e4m3, [head][slot][dim] each), then one exponent byte
+// per K row and one per V row ([head][slot]): row value = e4m3 * 2^(byte - 127).  Exponents follow the rows so that a
+// page is one run of bytes (copy-on-write, storage tier) and 16 keys of a head have theirs in one 16-byte vector.
+struct Pool8Layout {
+    int64_t plane, exp_plane, block, layer;
+    int num_kv_heads, page_size, head_dim, max_pages;
+    __host__ __device__ static Pool8Layout make(int hkv, int page, int d, int max_pages) {
+        Pool8Layout l;
+        l.plane = (int64_t)hkv * page * d;
+        l.exp_plane = (int64_t)hkv * page;
+        l.block = 2 * (l.plane + l.exp_plane);
+        l.layer = (int64_t)max_pages * l.block;
+        l.num_kv_heads = hkv;
+        l.page_size = page;
+        l.head_dim = d;
+        l.max_pages = max_pages;
+        return l;
+    }
+    __host__ __device__ int64_t block_of(int lay, int page) const { return lay * layer + page * block; }
+    // bytes from the block's start
+    __host__ __device__ int64_t row(int kv, int head, int slot) const {
+        return kv * plane + ((int64_t)head * page_size + slot) * head_dim;
+    }
+    __host__ __device__ int64_t exponent(int kv, int head, int slot) const {
+        return 2 * plane + kv * exp_plane + (int64_t)head * page_size + slot;
+    }
+};
+
+// Smallest e with |x| <= 448 * 2^e, for a finite fp32 |x| given by its bits; 448 = 1.75 * 2^8.  Held within -127 .. 120
+// (fp32 reaches no further up; rows below 2^-118 lose subnormal bits).
+__host__ __device__ __forceinline__ int e4m3_row_exponent(uint32_t abs_bits) {
+    const int e = (int)(abs_bits >> 23) - 127 - 8 + ((abs_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -127 ? -127 : e;
+}
+// 2^e for -127 <= e <= 127
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(e < -126 ? 0x00400000u : (uint32_t)(e + 127) << 23); }
+
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(two_bytes));
+    return r;
+}
+// bytes: lo in the lower one.  Values beyond 448 and infinities become 448, NaN stays NaN.
+__device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float lo, float hi) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 h;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %2, %1;\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
 template <typename T>
 struct Elem;
 template <>

@@ -209,6 +209,7 @@ bool PageStore::swap_in(int seq, int logical, int page) {
     else if (!read_file(path, staging_))
         return false;
     if (!copy_in(staging_, page)) return false;
+    swapped_in_.push_back(page);
     unlink(path.c_str());                            // the pool holds the only copy again (the reference leaves the file)
     bytes_in += (int64_t)file_bytes();
     return true;

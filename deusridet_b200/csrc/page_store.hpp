@@ -66,11 +66,18 @@ public:
     bool is_prefetched(int seq, int logical);
     void drain();                                   // waits for queued prefetches
 
+    // Pages that swap_in has filled since the last call (their page bounds are stale).
+    void take_swapped_in(std::vector<int>* pages) {
+        pages->swap(swapped_in_);
+        swapped_in_.clear();
+    }
+
     std::string path_for(int seq, int logical) const;
     size_t file_bytes() const { return (size_t)num_layers_ * page_bytes_; }
     int64_t bytes_out = 0, bytes_in = 0, prefetch_hits = 0, writes_deferred = 0, write_failures = 0;
 
 private:
+    std::vector<int> swapped_in_;
     std::string dir_;
     char* pool_ = nullptr;
     int num_layers_ = 0;

@@ -32,12 +32,18 @@ def _stream(stream) -> Optional[int]:
 
 class PagedKVEngine:
     def __init__(self, *, num_layers: int, num_q_heads: int, num_kv_heads: int, head_dim: int, page_size: int,
-                 dtype: str = "bf16", rotary_dim: Optional[int] = None, rope_theta: float = 10000.0,
+                 dtype: str = "bf16", kv_dtype: Optional[str] = None, rotary_dim: Optional[int] = None, rope_theta: float = 10000.0,
                  max_pages: int = 0, budget_bytes: int = 0, max_seqs: int = 1, max_pages_per_seq: int = 0,
                  device: int = 0, stream_evict: bool = False):
         self.lib = capi.load_library()
-        self.geom = Geometry(num_layers, num_q_heads, num_kv_heads, head_dim, page_size,
-                             capi.F16 if dtype in ("f16", "fp16") else capi.BF16,
+        if kv_dtype not in (None, "e4m3"):
+            raise ValueError(f"kv_dtype must be None (the pool has the type of Q) or 'e4m3', not {kv_dtype!r}")
+        f16 = dtype in ("f16", "fp16")
+        if kv_dtype == "e4m3":
+            pool_dtype = capi.F16_KV_E4M3 if f16 else capi.BF16_KV_E4M3
+        else:
+            pool_dtype = capi.F16 if f16 else capi.BF16
+        self.geom = Geometry(num_layers, num_q_heads, num_kv_heads, head_dim, page_size, pool_dtype,
                              head_dim if rotary_dim is None else rotary_dim, rope_theta)
         cfg = Config(budget_bytes, max_pages, max_seqs, max_pages_per_seq, device, 1 if stream_evict else 0)
         h = C.c_void_p()
@@ -192,6 +198,35 @@ class PagedKVEngine:
         """The planned pass with each entry's new token (position kv_len - 1 of the plan) appended in the same call."""
         check(self.lib.drkv_append_attend_decode_planned(self.h, layer, _ptr(k_src), _ptr(v_src), _ptr(q), _ptr(out),
                                                          scale, _stream(stream)))
+    # ---- page-sparse decode attention ------------------------------------------------------------
+    def page_bounds_enable(self, stream=None) -> None:
+        """Keeps channel bounds of every page's keys from now on (and scans the pages that exist)."""
+        check(self.lib.drkv_page_bounds_enable(self.h, _stream(stream)))
+    def page_bounds(self):
+        """(bounds int8 [layer, page, kv_head, 2, head_dim], exponents int8 [layer, page, kv_head]), aliasing the engine's memory."""
+        import torch
+        g = self.geom
+        def view(ptr, shape):
+            class _Raw:
+                pass
+            raw = _Raw()
+            raw.__cuda_array_interface__ = {"shape": shape, "typestr": "|i1", "data": (ptr, False), "version": 2}
+            return torch.as_tensor(raw, device=f"cuda:{self.device}")
+        ptr = self.lib.drkv_page_bounds(self.h)
+        if not ptr:
+            raise capi.DrkvError(capi.ERR_STATE, "page bounds are not enabled")
+        shape = (g.num_layers, self.max_blocks(), g.num_kv_heads)
+        return view(ptr, shape + (2, g.head_dim)), view(self.lib.drkv_page_bound_exponents(self.h), shape)
+    def select_pages(self, layer, n_seq, d_rows, d_kv_len, max_kv_len, q, top_pages, first_pages, last_pages, d_sel,
+                     stream=None) -> None:
+        """The best top_pages pages per sequence and KV head into d_sel (int32 [n_seq, num_kv_heads, top_pages])."""
+        check(self.lib.drkv_select_pages(self.h, layer, n_seq, _ptr(d_rows), _ptr(d_kv_len), max_kv_len, _ptr(q), top_pages,
+                                         first_pages, last_pages, _ptr(d_sel), _stream(stream)))
+    def attend_selected(self, layer, n_seq, d_rows, d_kv_len, max_kv_len, d_sel, top_pages, q, out, scale, stream=None) -> None:
+        """Decode attention over the listed pages only."""
+        check(self.lib.drkv_attend_selected(self.h, layer, n_seq, _ptr(d_rows), _ptr(d_kv_len), max_kv_len, _ptr(d_sel),
+                                            top_pages, _ptr(q), _ptr(out), scale, _stream(stream)))
+
     # ---- storage tier (KVSwapper + CacheManager swap paths) -----------------------------------
     def tier_enable(self, directory: str) -> None: check(self.lib.drkv_tier_enable(self.h, directory.encode()))
     def tier_disable(self) -> None: check(self.lib.drkv_tier_disable(self.h))

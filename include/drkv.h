@@ -26,6 +26,8 @@
  *       + head * page_size * head_dim + slot * head_dim + d
  *   kv_plane = num_kv_heads * page_size * head_dim, block_stride = 2 * kv_plane,
  *   layer_stride = max_pages * block_stride.
+ * An 8-bit pool has, in bytes, blocks of 2 * kv_plane + 2 * num_kv_heads * page_size: the K plane and the V plane as above,
+ * then one exponent byte (e + 127) per K row and one per V row, [head][slot].
  */
 #ifndef DRKV_H_
 #define DRKV_H_
@@ -49,7 +51,17 @@ typedef enum drkv_status {
     DRKV_ERR_CAPACITY = -6     /* position beyond the table, too many sequences, scratch too small */
 } drkv_status;
 
-enum { DRKV_DTYPE_F16 = 0, DRKV_DTYPE_BF16 = 1 };
+/* F16 and BF16: one type for Q, the K and V sources, the outputs and the pool, as in the reference.  The KV_E4M3 types keep
+ * the pool in 8 bits: rows are quantised as they are appended (drkv_append_rope, drkv_append_rope_chunk, the decode steps
+ * with append, drkv_seq_inject) and read back by decode attention, prefill attention and drkv_seq_extract.  A row, one
+ * token's K or V of one KV head, has e = the smallest integer with max|x| <= 448 * 2^e (held within -127..120) and stores
+ * x * 2^-e rounded to e4m3 (nearest even); it stands for those values times 2^e.  Infinities saturate, NaN stays NaN, and
+ * neither counts towards the maximum; K is rotated in fp32 before it is rounded.  drkv_seq_extract returns the values
+ * rounded to Q's type, which holds them exactly except below fp16's steps and beyond its range.  No counterpart in the reference.
+ * With an 8-bit pool the planned decode pass reads every sequence by itself, and these calls are refused
+ * (DRKV_ERR_INVALID): drkv_attend_partial, drkv_exchange_create, drkv_scorer_enable, drkv_set_prefill_on_decode_kernel(1)
+ * and the raw-pointer drkv_k_* functions. */
+enum { DRKV_DTYPE_F16 = 0, DRKV_DTYPE_BF16 = 1, DRKV_DTYPE_F16_KV_E4M3 = 2, DRKV_DTYPE_BF16_KV_E4M3 = 3 };
 
 /* Runtime geometry.  The reference fixes these at compile time (PagedKVConfig,
  * src/memoria/block_pool.h:34-52) or in process-wide statics (ModelConfig,
@@ -60,7 +72,7 @@ typedef struct drkv_geometry {
     int32_t num_kv_heads;
     int32_t head_dim;      /* 64, 128 or 256 */
     int32_t page_size;     /* tokens per page, a multiple of 16 */
-    int32_t dtype;         /* DRKV_DTYPE_* : storage type of Q, K, V, out and the pool */
+    int32_t dtype;         /* DRKV_DTYPE_* : type of Q, K, V and out, and of the pool */
     int32_t rotary_dim;    /* leading dims of each K head that RoPE rotates (0 = none) */
     float rope_theta;
 } drkv_geometry;
@@ -267,6 +279,36 @@ DRKV_API int drkv_attend_decode_planned(drkv_engine* e, int layer, const void* q
  * page and attends over them. */
 DRKV_API int drkv_append_attend_decode_planned(drkv_engine* e, int layer, const void* k_src, const void* v_src,
                                                const void* q, void* out, float scale, void* stream);
+/* ---- page-sparse decode attention --------------------------------------------------------------
+ * For long contexts: cheap bounds of every page's keys score the pages for each query, and attention reads only the best.
+ * No counterpart in the reference (its importance scores guide eviction, importance_scorer.h:25-67).
+ * Bounds of a (layer, page, KV head), int8: b_max[d] = ceil(max k[d] / 2^e), b_min[d] = floor(min k[d] / 2^e) over the keys of
+ * the page, e the smallest integer with max|k| <= 127 * 2^e (held within -126..121); NaN keys are ignored.
+ * From drkv_page_bounds_enable on, every call of this engine that writes keys keeps them: a page starts anew when its slot
+ * 0 is written and is widened by every other write, copies on write take them along, pages from the storage tier are
+ * scanned.  The call itself scans every slot of every page (calling it again does so again: for a host that has written
+ * through drkv_pool_ptr).  Bounds may be wider than a page's keys, never narrower.  Costs 1 / page_size of a 16-bit pool. */
+DRKV_API int drkv_page_bounds_enable(drkv_engine* e, void* stream);
+/* Device memory of the bounds, [layer][page][kv_head][b_max: head_dim, b_min: head_dim], and of their exponents,
+ * [layer][page][kv_head]; NULL before drkv_page_bounds_enable. */
+DRKV_API const int8_t* drkv_page_bounds(const drkv_engine* e);
+DRKV_API const int8_t* drkv_page_bound_exponents(const drkv_engine* e);
+/* For every sequence of the batch and every KV head the logical pages its query heads should read:
+ * d_sel[n_seq][num_kv_heads][top_pages], ascending, -1 behind the last.  All resident pages below kv_len if there are at most
+ * top_pages of them; else the first first_pages and the last last_pages logical pages (where resident) and the best scored
+ * (ties: the lower page).  With q8_h = rint(q_h / 2^f), f the smallest integer with max|q_h| <= 127 * 2^f, a page's score is the
+ * largest over the KV head's query heads of 2^(e + f) * sum_d (q8[d] > 0 ? q8[d] * b_max[d] : q8[d] * b_min[d]).
+ * q, d_rows, d_kv_len and max_kv_len as in drkv_attend_decode; first_pages + last_pages <= top_pages. */
+DRKV_API int drkv_select_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
+                               int max_kv_len, const void* q, int top_pages, int first_pages, int last_pages, int32_t* d_sel,
+                               void* stream);
+/* drkv_attend_decode over the listed pages only, of either kind of pool.  d_sel[n_seq][num_kv_heads][top_pages] need not come
+ * from drkv_select_pages: of each list the first min(top_pages, ceil(kv_len / page_size)) entries are read; entries that are
+ * negative, beyond the sequence or not resident contribute nothing, a page listed twice counts twice.  Keys at or
+ * beyond kv_len are not seen.  Rows without any visible key are left as they are. */
+DRKV_API int drkv_attend_selected(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
+                                  int max_kv_len, const int32_t* d_sel, int top_pages, const void* q, void* out, float scale,
+                                  void* stream);
 /* ---- storage tier behind the pool --------------------------------------------------------------
  * KVSwapper (kv_swapper.h:52-120, kv_swapper.cpp:179-300) and CacheManager's swap paths
  * (cache_manager.cpp:132-141, 215-292): with a tier enabled, a page that a sequence evicts from
