@@ -6,9 +6,10 @@
 //
 // Split: the keys of all (sequence, KV head) pairs form one line of 16-key groups.  Every warp of a persistent grid takes
 // an equal stretch of it (at least kMinShare groups), whatever the lengths are: ragged batches need no queue and no
-// tail.  A pair that lies inside one stretch is finished by its warp; one that is cut leaves a partial (m, l, o) per
-// stretch, at most two a warp, and a second small kernel merges them in a fixed order (results do not depend on timing).
-// Warps of one CTA take stretches far apart, so that a short line still spreads over all SMs.
+// tail.  A pair that lies inside one stretch is finished by its warp; one that is cut leaves a piece (m, l, o) per stretch,
+// at most two a warp, and a second small kernel merges them in a fixed order (results do not depend on timing).  Warps of
+// one CTA take stretches far apart, so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and
+// then by the last CTA to arrive, took 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end.
 //
 // A warp brings its groups into a private ring of shared memory by cp.async (16 bytes a lane, L1 bypassed), kStages - 1
 // groups ahead, and reads them as matrix operands without ldmatrix: contraction order is free, so a lane takes whole
@@ -33,17 +34,18 @@ namespace drkv {
 
 namespace {
 
-constexpr int kMinShare = 4;          // 16-key groups: shorter stretches cost more in partials than they save
+constexpr int kMinShare = 2;          // 16-key groups: shorter stretches cost more in partials than they save
 constexpr float kNoKey = -1.0e30f;    // running maximum before any key
 
 // Warps per CTA (one CTA per SM) and groups in a warp's ring.
-template <bool POOL8, int D> struct Ring;
-template <> struct Ring<true, 64>   { static constexpr int kWarps = 16, kStages = 4; };   // 132 KB
-template <> struct Ring<true, 128>  { static constexpr int kWarps = 16, kStages = 3; };   // 198 KB
-template <> struct Ring<true, 256>  { static constexpr int kWarps = 8, kStages = 3; };    // 197 KB
-template <> struct Ring<false, 64>  { static constexpr int kWarps = 16, kStages = 3; };   // 192 KB
-template <> struct Ring<false, 128> { static constexpr int kWarps = 8, kStages = 3; };    // 192 KB
-template <> struct Ring<false, 256> { static constexpr int kWarps = 6, kStages = 2; };    // 192 KB
+template <bool POOL8, int D, int NQ> struct Ring;
+template <int NQ> struct Ring<true, 64, NQ>   { static constexpr int kWarps = 16, kStages = 4; };   // 132 KB
+template <> struct Ring<true, 128, 1>         { static constexpr int kWarps = 16, kStages = 3; };   // 198 KB
+template <> struct Ring<true, 128, 2>         { static constexpr int kWarps = 8, kStages = 5; };    // 165 KB
+template <int NQ> struct Ring<true, 256, NQ>  { static constexpr int kWarps = 8, kStages = 3; };    // 197 KB
+template <int NQ> struct Ring<false, 64, NQ>  { static constexpr int kWarps = 16, kStages = 3; };   // 192 KB
+template <int NQ> struct Ring<false, 128, NQ> { static constexpr int kWarps = 8, kStages = 3; };    // 192 KB
+template <int NQ> struct Ring<false, 256, NQ> { static constexpr int kWarps = 6, kStages = 2; };    // 192 KB
 
 // A tile is 16 rows of ROWB bytes in shared memory; chunks of 16 bytes are permuted so that both access patterns are free
 // of bank conflicts: rows (g) x chunks (t) for K, rows (2t) x chunks (g) for V, g = lane / 4, t = lane % 4.
@@ -69,8 +71,11 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
     return v;
 }
-// 16 bytes from global to shared memory, zeros where !live
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool live) {
+// 16 bytes from global to shared memory; the second form writes zeros where !live
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool live) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -95,36 +100,41 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The work split, left by the first kernel for the second: share, then the line's prefix sums over the sequences.
+// What the first kernel leaves for the second, in front of the pieces.
 struct Split {
-    int share;
-    int cum[kMaxDecodeSeqs + 1];
+    int share, pad[3];
+    int cum[kMaxPagesSeqs + 4];        // prefix sums of the line over the sequences
 };
-constexpr size_t kSplitFloats = (sizeof(Split) + 255) / 256 * 64;
+constexpr size_t kSplitFloats = sizeof(Split) / 4;
 
-struct PartialView {                   // slot = 2 * warp + (the stretch's first piece ? 0 : 1), row = head of the group
-    float *o, *m, *l;
-    __host__ __device__ PartialView(float* scratch, size_t slots, int group, int d) {
+// Pieces: slot = 2 * warp + (the stretch begins inside the pair ? 0 : 1), row = slot * group + head of the group;
+// un-normalised sums [row][D], then maxima (log2 domain) and sums of weights as pairs [row].
+struct Pieces {
+    float* o;
+    float2* ml;
+    __host__ __device__ Pieces(float* scratch, int n_warps, int group, int d) {
         o = scratch + kSplitFloats;
-        m = o + slots * group * d;
-        l = m + slots * group;
+        ml = reinterpret_cast<float2*>(o + 2 * (size_t)n_warps * group * d);
     }
 };
 
-// Groups of a pair of sequence b.  A list has at most as many entries as the sequence has pages.
-__device__ __forceinline__ int pair_groups(const AttendPagesParams& p, int b, bool list) {
-    int len = __ldg(p.kv_len + b);
-    len = min(len, p.max_kv_len);
-    const int row = __ldg(p.rows + b);
-    if (len <= 0 || row < 0 || row >= p.max_rows) return 0;
+// Groups of a pair of a sequence.  A list has at most as many entries as the sequence has pages.
+__device__ __forceinline__ int pair_groups(const AttendPagesParams& p, int len, bool list) {
+    if (len <= 0) return 0;
     if (!list) return (len + 15) >> 4;
     const int pages = (len - 1) / p.page_size + 1;
     return min(pages, p.list_len) * (p.page_size >> 4);
 }
 
+// One group of the line as its warp needs it; a warp keeps the next 64 in shared memory.
+struct alignas(16) Group {
+    int pair, valid;                   // visible keys (0: nothing to read)
+    int page, row;                     // pool page; first row in its plane
+};
+
 template <bool POOL8, typename T, int D, int NQ, bool LIST>
-__global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_kernel(const AttendPagesParams p) {
-    constexpr int WARPS = Ring<POOL8, D>::kWarps, STAGES = Ring<POOL8, D>::kStages, THREADS = WARPS * 32;
+__global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pages_kernel(const AttendPagesParams p) {
+    constexpr int WARPS = Ring<POOL8, D, NQ>::kWarps, STAGES = Ring<POOL8, D, NQ>::kStages, THREADS = WARPS * 32;
     using TM = typename std::conditional<POOL8, __half, T>::type;           // matrix operand type
     constexpr bool F16 = std::is_same<TM, __half>::value;
     constexpr bool LO = !(POOL8 && std::is_same<T, __nv_bfloat16>::value);
@@ -134,24 +144,33 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
     constexpr int KCH = CPR / 4;                                            // K chunks a lane reads of a row
     constexpr int EPL = POOL8 ? (D == 64 ? 8 : 16) : 8;                     // V elements a lane reads of a row at once
     constexpr int VCH = D / (8 * EPL);
-    constexpr int WS = F16 ? 15 : 0;                                        // weights carry 2^WS
+    // Weights carry 2^WS and may exceed their maximum's by 2^kSlack before the maximum follows: at most 2^15 in f16.
+    constexpr float kSlack = 8.f;
+    constexpr int WS = F16 ? 7 : 0;
     constexpr uint32_t FULL = 0xffffffffu;
 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int s_warp_tot[WARPS];
-    __shared__ int2 s_meta[WARPS][STAGES];                                  // pair, visible keys of the group
+    __shared__ Group s_groups[WARPS][64];
     int* cum = reinterpret_cast<int*>(smem + WARPS * STAGES * SLOT);        // [n_seq + 1]
+    int* s_len = cum + p.n_seq + 1;                                         // [n_seq] keys, 0 where nothing is read
+    int* s_row = s_len + p.n_seq;                                           // [n_seq] table rows
 
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    pdl_wait();
-    pdl_launch_dependents();
+    // Lengths, rows and tables were written further back than the kernel directly in front (attend_decode_kernel has the
+    // same rule): the split and the first page ids are worked out under that kernel's tail.  A page list may be its output.
 
     // ---- prefix sums of the line over the sequences ----
     {
         const int per = (p.n_seq + THREADS - 1) / THREADS;
         const int lo = min(tid * per, p.n_seq), hi = min(lo + per, p.n_seq);
         int local = 0;
-        for (int b = lo; b < hi; b++) local += pair_groups(p, b, LIST) * p.num_kv_heads;
+        for (int b = lo; b < hi; b++) {
+            const int row = __ldg(p.rows + b), len = min(__ldg(p.kv_len + b), p.max_kv_len);
+            s_row[b] = row;
+            s_len[b] = row >= 0 && row < p.max_rows ? len : 0;
+            local += pair_groups(p, s_len[b], LIST) * p.num_kv_heads;
+        }
         int incl = local;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -164,95 +183,132 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
         for (int i = 0; i < w; i++) run += s_warp_tot[i];
         for (int b = lo; b < hi; b++) {
             cum[b] = run;
-            run += pair_groups(p, b, LIST) * p.num_kv_heads;
+            run += pair_groups(p, s_len[b], LIST) * p.num_kv_heads;
         }
         if (tid == THREADS - 1) cum[p.n_seq] = run;
         __syncthreads();
     }
-    const int total = cum[p.n_seq];
-    const int n_warps = (int)gridDim.x * WARPS;
+    const int total = cum[p.n_seq], n_warps = (int)gridDim.x * WARPS;
     const int share = max(kMinShare, (total + n_warps - 1) / n_warps);
-    if (blockIdx.x == 0) {
-        Split* split = reinterpret_cast<Split*>(p.scratch);
-        if (tid == 0) split->share = share;
-        for (int b = tid; b <= p.n_seq; b += THREADS) split->cum[b] = cum[b];
-    }
     const int gw = w * (int)gridDim.x + (int)blockIdx.x;
     const int64_t lo64 = (int64_t)gw * share;
-    if (lo64 >= total) return;                                              // no block-wide barrier below
-    const int lo = (int)lo64, n = min(share, total - lo);
+    const int lo = lo64 < total ? (int)lo64 : total, n = min(share, total - lo);
 
-    // ---- where a group of the line lies: lane i describes group (window's first) + i ----
-    struct Where { int pair, tok, valid, page; };
-    auto locate = [&](int idx) -> Where {
-        Where r{-1, 0, 0, -1};
-        if (idx >= n) return r;
-        const int f = lo + idx;
+    // The pair that holds a group of the line, and where it starts and ends.
+    struct Span { int pair, start, end; };
+    auto pair_at = [&](int f) -> Span {
         int b = 0, e = p.n_seq;                                             // largest b with cum[b] <= f
         while (e - b > 1) {
             const int mid = (b + e) >> 1;
             if (cum[mid] <= f) b = mid; else e = mid;
         }
-        const int groups = (cum[b + 1] - cum[b]) / p.num_kv_heads;
-        const int rem = f - cum[b], h = rem / groups, i = rem - h * groups;
-        r.pair = b * p.num_kv_heads + h;
-        const int len = min(__ldg(p.kv_len + b), p.max_kv_len);
-        const int per_page = p.page_size >> 4;
-        int logical = i / per_page;
-        const int sub = i - logical * per_page;
-        if (LIST) logical = __ldg(p.list + (int64_t)r.pair * p.list_len + logical);
-        if (logical < 0 || logical >= p.table_stride) return r;
-        const int64_t tok = (int64_t)logical * p.page_size + sub * 16;
-        if (tok >= len) return r;
-        r.tok = (int)tok;
-        r.page = __ldg(p.tables + (int64_t)__ldg(p.rows + b) * p.table_stride + logical);
-        if (r.page >= p.max_pages) {
-            atomicExch(p.error_word, (int)KERR_BAD_PAGE);
-            r.page = -1;
-        }
-        if (r.page >= 0) r.valid = min(16, len - r.tok);
-        return r;
+        const int groups = (cum[b + 1] - cum[b]) / p.num_kv_heads, h = (f - cum[b]) / groups;
+        return Span{b * p.num_kv_heads + h, cum[b] + h * groups, cum[b] + (h + 1) * groups};
     };
-    Where cur = locate(lane), next = cur;
-    const uint32_t ring = smem_u32(smem) + w * STAGES * SLOT;
 
+    // ---- the groups ahead: lane i works out group (window's first) + i; the look-ups are spread over the window before ----
+    int ahead_pair = -1, ahead_in = 0, ahead_logical = -1, ahead_page = -1;
+    const int per_page = p.page_size >> 4;
+    auto locate_pair = [&](int idx) {                                       // step 1: pair and list entry
+        ahead_pair = -1;
+        ahead_logical = -1;
+        if (idx < n) {
+            const Span s = pair_at(lo + idx);
+            ahead_pair = s.pair;
+            const int i = lo + idx - s.start;
+            ahead_logical = i / per_page;
+            ahead_in = i - ahead_logical * per_page;
+            if (LIST) ahead_logical = __ldg(p.list + (int64_t)s.pair * p.list_len + ahead_logical);
+        }
+    };
+    auto locate_page = [&]() {                                              // step 2: page
+        ahead_page = -1;
+        if (ahead_pair >= 0 && ahead_logical >= 0 && ahead_logical < p.table_stride)
+            ahead_page = __ldg(p.tables + (int64_t)s_row[ahead_pair / p.num_kv_heads] * p.table_stride + ahead_logical);
+    };
+    auto locate_done = [&](int idx) {                                       // step 3: into the warp's list
+        Group r{ahead_pair, 0, 0, 0};
+        if (ahead_page >= p.max_pages) {
+            atomicExch(p.error_word, (int)KERR_BAD_PAGE);
+            ahead_page = -1;
+        }
+        if (ahead_page >= 0) {
+            const int b = ahead_pair / p.num_kv_heads, h = ahead_pair - b * p.num_kv_heads;
+            const int len = s_len[b];
+            const int64_t tok = (int64_t)ahead_logical * p.page_size + ahead_in * 16;
+            if (tok < len) r.valid = min(16, (int)(len - tok));
+            r.page = ahead_page;
+            r.row = h * p.page_size + ahead_in * 16;
+        }
+        s_groups[w][idx & 63] = r;
+    };
+    if (LIST) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
+    locate_pair(lane);
+    locate_page();
+    locate_done(lane);
+    __syncwarp();
+    if (!LIST) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
+    if (blockIdx.x == 0) {
+        Split* split = reinterpret_cast<Split*>(p.scratch);
+        if (tid == 0) split->share = share;
+        for (int b = tid; b <= p.n_seq; b += THREADS) split->cum[b] = cum[b];
+    }
+    if (n <= 0) return;                                                     // no block-wide barrier below
+
+    const uint32_t ring = smem_u32(smem) + w * STAGES * SLOT;
+    const uint8_t* lane_src = p.pool + 16 * lane;
+    // a lane's chunks of a tile are 32 apart: c = lane + 32 j, row = c / CPR; in the permuted tile the j part of the row
+    // contributes a constant XOR and a constant offset to the lane's own place
+    const uint32_t lane_dst = tile_off<ROWB>(lane / CPR, lane % CPR);
     auto issue = [&](int idx) {                                             // requests group idx of the stretch
         const int wl = idx & 31;
-        if (wl == 0) {
-            if (idx > 0) cur = next;
-            if (idx + 32 < n) next = locate(idx + 32 + lane);               // used 32 groups from now
-        }
-        const int pair = __shfl_sync(FULL, cur.pair, wl), tok = __shfl_sync(FULL, cur.tok, wl);
-        const int valid = __shfl_sync(FULL, cur.valid, wl), page = __shfl_sync(FULL, cur.page, wl);
-        const int stage = idx % STAGES;
-        if (lane == 0) s_meta[w][stage] = make_int2(pair, valid);
-        if (valid > 0) {
-            const uint32_t dst = ring + stage * SLOT;
-            const int h = pair % p.num_kv_heads;
-            const int64_t row0 = (int64_t)h * p.page_size + tok % p.page_size;
-            const uint8_t* block = p.pool + (int64_t)page * p.block_bytes;
-            const uint8_t* k = block + row0 * ROWB;
-            const uint8_t* v = k + p.plane_bytes;
-#pragma unroll
-            for (int c = lane; c < 16 * CPR; c += 32) {
-                const int row = c / CPR;
-                const uint32_t off = tile_off<ROWB>(row, c % CPR);
-                copy16(dst + off, k + 16 * c, row < valid);
-                copy16(dst + TILE + off, v + 16 * c, row < valid);          // hidden rows are zeros: they meet zero weights
+        const int nx = (idx & ~31) + 32 + lane;
+        if ((idx & ~31) + 32 < n) {                                         // the next window's look-ups
+            if (wl == 0) locate_pair(nx);
+            if (wl == 8) locate_page();
+            if (wl == 16) {
+                locate_done(nx);
+                __syncwarp();
             }
-            if (POOL8 && lane < 2) copy16(dst + 2 * TILE + 16 * lane, block + 2 * p.plane_bytes + lane * p.exp_plane_bytes + row0, true);
         }
+        const Group gr = s_groups[w][idx & 63];
+        if (gr.valid == 0) return;
+        const uint32_t dst = ring + (idx % STAGES) * SLOT;
+        const int64_t block = gr.page * p.block_bytes;
+        const uint8_t* k = lane_src + block + (int64_t)gr.row * ROWB;
+        const uint8_t* v = k + p.plane_bytes;
+#pragma unroll
+        for (int j = 0; j < CPR / 2; j++) {
+            const int row_j = 32 * j / CPR;                                 // rows below 16, constant
+            const uint32_t flip = tile_off<ROWB>(row_j, 0) & 127u, skip = tile_off<ROWB>(row_j, 0) & ~127u;
+            const uint32_t off = (lane_dst ^ flip) + skip;
+            if (gr.valid == 16) {
+                copy16(dst + off, k + 512 * j);
+                copy16(dst + TILE + off, v + 512 * j);
+            } else {                                                        // hidden rows are zeros: they meet zero weights
+                const bool see = (lane + 32 * j) / CPR < gr.valid;
+                copy16_or_zero(dst + off, k + 512 * j, see);
+                copy16_or_zero(dst + TILE + off, v + 512 * j, see);
+            }
+        }
+        if (POOL8 && lane < 2)                                              // 16 exponents of K, 16 of V
+            copy16(dst + 2 * TILE + 16 * lane, p.pool + block + 2 * p.plane_bytes + lane * p.exp_plane_bytes + gr.row);
     };
 
     // ---- state of the pair being attended ----
     uint32_t qf[NQ][KSTEPS][2];
     float qs[NQ][2];                                                        // score factor of heads 2t and 2t + 1
     float o[NQ][MT][4], m[NQ][2], l[NQ][2];
-    int big_e = -127, cur_pair = -1, seg_begin = 0;
+    int big_e = 0, cur_pair = -1;                                           // big_e: V exponent byte the weights are relative to
 
-    auto begin_pair = [&](int pair, int f) {
+    auto begin_pair = [&](int pair) {
         cur_pair = pair;
-        seg_begin = f;
         const int b = pair / p.num_kv_heads, h = pair - b * p.num_kv_heads;
         const T* q = reinterpret_cast<const T*>(p.q) + ((int64_t)b * p.num_kv_heads + h) * p.group * D;
 #pragma unroll
@@ -310,17 +366,17 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) o[nq][mt][0] = o[nq][mt][1] = o[nq][mt][2] = o[nq][mt][3] = 0.f;
         }
-        big_e = -127;
+        big_e = 0;
     };
 
-    auto end_pair = [&](int f_end) {
+    const Pieces pieces(p.scratch, n_warps, p.group, D);
+    auto end_pair = [&]() {
         const int b = cur_pair / p.num_kv_heads, h = cur_pair - b * p.num_kv_heads;
         const int groups = (cum[b + 1] - cum[b]) / p.num_kv_heads;
         const int start = cum[b] + h * groups;
-        const bool whole = seg_begin == start && f_end == start + groups;
-        const PartialView parts(p.scratch, 2 * (size_t)n_warps, p.group, D);
-        const int64_t slot = 2 * (int64_t)gw + (seg_begin == lo ? 0 : 1);
-        const float unit = POOL8 ? exp2_int(big_e) : 1.f;
+        const bool whole = start >= lo && start + groups <= lo + n;
+        const int64_t row0 = (2 * (int64_t)gw + (start > lo ? 1 : 0)) * p.group;
+        const float unit = POOL8 ? exp2_int(big_e - 127) : 1.f;
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -330,37 +386,33 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
                 sum += __shfl_xor_sync(FULL, sum, 8);
                 sum += __shfl_xor_sync(FULL, sum, 16);
                 const int head = nq * 8 + 2 * t + c;
-                if (head >= p.group) continue;
-                const float f = (whole ? 1.f / sum : 1.f) * (F16 ? 0x1p-15f : 1.f);
-                const int64_t row = slot * p.group + head;
-                if (!whole && g == 0) {
-                    parts.m[row] = m[nq][c];
-                    parts.l[row] = sum;
-                }
+                if (head < p.group) {
+                    const float f = (whole ? 1.f / sum : 1.f) * (F16 ? 0x1p-7f : 1.f);
+                    if (!whole && g == 0) pieces.ml[row0 + head] = make_float2(m[nq][c], sum);
 #pragma unroll
-                for (int j = 0; j < VCH; j++) {
-                    const int dim = (g + 8 * j) * EPL;
-                    float x[EPL];
+                    for (int j = 0; j < VCH; j++) {
+                        const int dim = (g + 8 * j) * EPL;
+                        float x[EPL];
 #pragma unroll
-                    for (int i = 0; i < EPL / 2; i++) {
-                        x[2 * i] = o[nq][j * (EPL / 2) + i][c] * f * unit;
-                        x[2 * i + 1] = o[nq][j * (EPL / 2) + i][2 + c] * f * unit;
-                    }
-                    if (whole) {
-                        if (!(sum != 0.f)) continue;                        // no visible key: the row stays as it is
-                        T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)b * p.num_kv_heads + h) * p.group + head) * D + dim;
-#pragma unroll
-                        for (int i = 0; i < EPL; i += 8) {
-                            Vec16 v;
-#pragma unroll
-                            for (int k = 0; k < 4; k++) v.w[k] = Elem<T>::pack2(x[i + 2 * k], x[i + 2 * k + 1]);
-                            stg16(dst + i, v);
+                        for (int i = 0; i < EPL / 2; i++) {
+                            x[2 * i] = o[nq][j * (EPL / 2) + i][c] * f * unit;
+                            x[2 * i + 1] = o[nq][j * (EPL / 2) + i][2 + c] * f * unit;
                         }
-                    } else {
-                        float* dst = parts.o + row * D + dim;
+                        if (!whole) {
+                            float* dst = pieces.o + (row0 + head) * D + dim;
 #pragma unroll
-                        for (int i = 0; i < EPL; i += 4)
-                            *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                            for (int i = 0; i < EPL; i += 4)
+                                *reinterpret_cast<float4*>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                        } else if (sum != 0.f) {                            // no visible key: the row stays as it is
+                            T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)b * p.num_kv_heads + h) * p.group + head) * D + dim;
+#pragma unroll
+                            for (int i = 0; i < EPL; i += 8) {
+                                Vec16 v;
+#pragma unroll
+                                for (int k = 0; k < 4; k++) v.w[k] = Elem<T>::pack2(x[i + 2 * k], x[i + 2 * k + 1]);
+                                stg16(dst + i, v);
+                            }
+                        }
                     }
                 }
             }
@@ -371,6 +423,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
         float s[NQ][4];
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) s[nq][0] = s[nq][1] = s[nq][2] = s[nq][3] = 0.f;
+        float s2[4] = {0.f, 0.f, 0.f, 0.f};                                 // one tile: two chains of dependent products
 #pragma unroll
         for (int i = 0; i < KCH; i++) {
             const uint4 ka = lds128(tile + tile_off<ROWB>(g, t + 4 * i)), kb = lds128(tile + tile_off<ROWB>(g + 8, t + 4 * i));
@@ -378,89 +431,109 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
             if (POOL8) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t a0 = e4m3x2_to_f16x2(a[j] & 0xffffu), a2 = e4m3x2_to_f16x2(a[j] >> 16);
-                    const uint32_t a1 = e4m3x2_to_f16x2(b[j] & 0xffffu), a3 = e4m3x2_to_f16x2(b[j] >> 16);
+                    uint32_t a0, a1, a2, a3;
+                    e4m3x4_to_f16x4(a[j], a0, a2);
+                    e4m3x4_to_f16x4(b[j], a1, a3);
 #pragma unroll
                     for (int nq = 0; nq < NQ; nq++)
-                        mma16816<TM>(s[nq], a0, a1, a2, a3, qf[nq][(4 * i + j) % KSTEPS][0], qf[nq][(4 * i + j) % KSTEPS][1]);
+                        mma16816<TM>(NQ == 1 && (j & 1) ? s2 : s[nq], a0, a1, a2, a3, qf[nq][(4 * i + j) % KSTEPS][0],
+                                     qf[nq][(4 * i + j) % KSTEPS][1]);
                 }
             } else {
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
                     for (int nq = 0; nq < NQ; nq++)
-                        mma16816<TM>(s[nq], a[2 * j], b[2 * j], a[2 * j + 1], b[2 * j + 1], qf[nq][(2 * i + j) % KSTEPS][0],
+                        mma16816<TM>(NQ == 1 && (j & 1) ? s2 : s[nq], a[2 * j], b[2 * j], a[2 * j + 1], b[2 * j + 1], qf[nq][(2 * i + j) % KSTEPS][0],
                                      qf[nq][(2 * i + j) % KSTEPS][1]);
             }
         }
-        const bool see0 = g < valid, see1 = g + 8 < valid;
-        float ks0 = 1.f, ks1 = 1.f;
-        int ev0 = 0, ev1 = 0, new_e = big_e;
-        if (POOL8) {
-            ks0 = exp2_int((int)lds8(tile + 2 * TILE + g) - 127);
-            ks1 = exp2_int((int)lds8(tile + 2 * TILE + g + 8) - 127);
-            ev0 = (int)lds8(tile + 2 * TILE + 16 + g) - 127;
-            ev1 = (int)lds8(tile + 2 * TILE + 24 + g) - 127;
-            new_e = max(big_e, __reduce_max_sync(FULL, max(see0 ? ev0 : -127, see1 ? ev1 : -127)));
-        }
-        float mx[NQ][2];
-        bool grow = new_e > big_e;
+        if (NQ == 1) {
 #pragma unroll
-        for (int nq = 0; nq < NQ; nq++) {
+            for (int k = 0; k < 4; k++) s[0][k] += s2[k];
+        }
+        // s * f is the score in the log2 domain.  A K row whose byte is 0 (everything below 2^-118) counts as zeros.
+        float f0[NQ][2], f1[NQ][2];
+        uint32_t ev0 = 0, ev1 = 0;
+        float ks0 = 1.f, ks1 = 1.f;
+        if (POOL8) {
+            ks0 = __uint_as_float(lds8(tile + 2 * TILE + g) << 23);
+            ks1 = __uint_as_float(lds8(tile + 2 * TILE + g + 8) << 23);
+            ev0 = lds8(tile + 2 * TILE + 16 + g);
+            ev1 = lds8(tile + 2 * TILE + 24 + g);
+        }
+        if (valid < 16) {                                                   // what lies behind the last key may be anything
+            if (g >= valid) ev0 = 0, ks0 = 0.f;
+            if (g + 8 >= valid) ev1 = 0, ks1 = 0.f;
+        }
+        // The maximum follows only when a score exceeds it by more than kSlack, and then in full: most groups need no
+        // reduction over the lanes.
+        bool grow = (int)max(ev0, ev1) > big_e;
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                s[nq][c] = see0 ? s[nq][c] * (ks0 * qs[nq][c]) : -INFINITY;
-                s[nq][2 + c] = see1 ? s[nq][2 + c] * (ks1 * qs[nq][c]) : -INFINITY;
-                float x = fmaxf(s[nq][c], s[nq][2 + c]);
-                x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
-                x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
-                x = fmaxf(x, __shfl_xor_sync(FULL, x, 16));
-                mx[nq][c] = fmaxf(m[nq][c], x);
-                grow |= mx[nq][c] > m[nq][c];
+                f0[nq][c] = POOL8 ? ks0 * qs[nq][c] : qs[nq][c];
+                f1[nq][c] = POOL8 ? ks1 * qs[nq][c] : qs[nq][c];
+                grow |= fmaxf(fmaf(s[nq][c], f0[nq][c], -m[nq][c]), fmaf(s[nq][2 + c], f1[nq][c], -m[nq][c])) > kSlack;
             }
-        }
         if (__any_sync(FULL, grow)) {
+            const int new_e = POOL8 ? max(big_e, __reduce_max_sync(FULL, (int)max(ev0, ev1))) : 0;
             // 2^(old - new E) in two factors: the difference may be 247
             const int de = big_e - new_e;
             const float e1 = exp2_int(max(de, -126)), e2 = exp2_int(max(de - max(de, -126), -126));
-#pragma unroll
-            for (int nq = 0; nq < NQ; nq++) {
-                const float f0 = fast_exp2(m[nq][0] - mx[nq][0]), f1 = fast_exp2(m[nq][1] - mx[nq][1]);
-                m[nq][0] = mx[nq][0];
-                m[nq][1] = mx[nq][1];
-                l[nq][0] *= f0;
-                l[nq][1] *= f1;
-                const float r0 = POOL8 ? f0 * e1 * e2 : f0, r1 = POOL8 ? f1 * e1 * e2 : f1;
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    o[nq][mt][0] *= r0;
-                    o[nq][mt][1] *= r1;
-                    o[nq][mt][2] *= r0;
-                    o[nq][mt][3] *= r1;
-                }
-            }
             big_e = new_e;
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float x = fmaxf(g < valid ? s[nq][c] * f0[nq][c] : -INFINITY, g + 8 < valid ? s[nq][2 + c] * f1[nq][c] : -INFINITY);
+                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 16));
+                    x = fmaxf(x, m[nq][c]);
+                    const float f = fast_exp2(m[nq][c] - x), r = POOL8 ? f * e1 * e2 : f;
+                    m[nq][c] = x;
+                    l[nq][c] *= f;
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        o[nq][mt][c] *= r;
+                        o[nq][mt][2 + c] *= r;
+                    }
+                }
         }
         // ---- weights ----
-        float vs0 = F16 ? 0x1p15f : 1.f, vs1 = vs0;
-        if (POOL8) {
-            vs0 = exp2_int(max(min(ev0, big_e) - big_e + WS, -127));
-            vs1 = exp2_int(max(min(ev1, big_e) - big_e + WS, -127));
+        float vs0 = F16 ? 0x1p7f : 1.f, vs1 = vs0;
+        if (POOL8) {                                                        // 2^(ev - E + WS), 0 below 2^-126
+            vs0 = __uint_as_float((uint32_t)max((int)ev0 - big_e + WS + 127, 0) << 23);
+            vs1 = __uint_as_float((uint32_t)max((int)ev1 - big_e + WS + 127, 0) << 23);
         }
         uint32_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
-            const float p00 = fast_exp2(s[nq][0] - m[nq][0]), p01 = fast_exp2(s[nq][1] - m[nq][1]);
-            const float p10 = fast_exp2(s[nq][2] - m[nq][0]), p11 = fast_exp2(s[nq][3] - m[nq][1]);
-            l[nq][0] += p00 + p10;
-            l[nq][1] += p01 + p11;
-            const uint32_t h0 = Elem<TM>::pack2(p00 * vs0, p01 * vs0), h1 = Elem<TM>::pack2(p10 * vs1, p11 * vs1);
+            float w0[2], w1[2];
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                w0[c] = fast_exp2(fmaf(s[nq][c], f0[nq][c], -m[nq][c]));
+                w1[c] = fast_exp2(fmaf(s[nq][2 + c], f1[nq][c], -m[nq][c]));
+            }
+            if (valid < 16) {
+                if (g >= valid) w0[0] = w0[1] = 0.f;
+                if (g + 8 >= valid) w1[0] = w1[1] = 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                l[nq][c] += w0[c] + w1[c];
+                w0[c] *= vs0;
+                w1[c] *= vs1;
+            }
+            const uint32_t h0 = Elem<TM>::pack2(w0[0], w0[1]), h1 = Elem<TM>::pack2(w1[0], w1[1]);
             pf[nq][0] = transpose8x8(h0);
             pf[nq][1] = transpose8x8(h1);
             if (LO) {
                 const float2 a = Elem<TM>::unpack2(h0), b = Elem<TM>::unpack2(h1);
-                pl[nq][0] = transpose8x8(Elem<TM>::pack2(p00 * vs0 - a.x, p01 * vs0 - a.y));
-                pl[nq][1] = transpose8x8(Elem<TM>::pack2(p10 * vs1 - b.x, p11 * vs1 - b.y));
+                pl[nq][0] = transpose8x8(Elem<TM>::pack2(w0[0] - a.x, w0[1] - a.y));
+                pl[nq][1] = transpose8x8(Elem<TM>::pack2(w1[0] - b.x, w1[1] - b.y));
             }
         }
         // ---- O^T += V^T P^T: keys 2t, 2t + 1, 2t + 8, 2t + 9; dims (g + 8 j) EPL + 0 .. EPL - 1 ----
@@ -498,8 +571,10 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
                     for (int half = 0; half < 2; half++) {
                         const uint32_t x = __byte_perm(v[0][i], v[1][i], half ? 0x7362 : 0x5140);
                         const uint32_t y = __byte_perm(v[2][i], v[3][i], half ? 0x7362 : 0x5140);
-                        pv(j * (EPL / 2) + 2 * i + half, e4m3x2_to_f16x2(x & 0xffffu), e4m3x2_to_f16x2(x >> 16),
-                           e4m3x2_to_f16x2(y & 0xffffu), e4m3x2_to_f16x2(y >> 16));
+                        uint32_t a0, a1, a2, a3;
+                        e4m3x4_to_f16x4(x, a0, a1);
+                        e4m3x4_to_f16x4(y, a2, a3);
+                        pv(j * (EPL / 2) + 2 * i + half, a0, a1, a2, a3);
                     }
                 } else {
                     pv(j * (EPL / 2) + i, __byte_perm(v[0][i], v[1][i], 0x5410), __byte_perm(v[0][i], v[1][i], 0x7632),
@@ -515,110 +590,132 @@ __global__ void __launch_bounds__(Ring<POOL8, D>::kWarps * 32, 1) attend_pages_k
         if (i < n) issue(i);
         copies_commit();
     }
-    for (int i = 0; i < n; i++) {
+    // (one place each for the start and the end of a pair: the code is long, and short launches pay for fetching it)
+    for (int i = 0; i <= n; i++) {
+        const int2 meta = *reinterpret_cast<const int2*>(&s_groups[w][i & 63]);   // pair, visible keys
+        if (i == n || meta.x != cur_pair) {
+            if (cur_pair >= 0) end_pair();
+            if (i == n) break;
+            begin_pair(meta.x);                                             // its query rows come while the keys do
+        }
         if (i + STAGES - 1 < n) issue(i + STAGES - 1);
         copies_commit();
         copies_wait<STAGES - 1>();
         __syncwarp();
-        const int2 meta = s_meta[w][i % STAGES];
-        if (meta.x != cur_pair) {
-            if (cur_pair >= 0) end_pair(lo + i);
-            begin_pair(meta.x, lo + i);
-        }
         if (meta.y > 0) attend_group(ring + (i % STAGES) * SLOT, meta.y);
         __syncwarp();                                                       // the slot is free for the next request
     }
-    end_pair(lo + n);
+    copies_wait<0>();
 }
 
-// One CTA per (query head, sequence): merges what the stretches left of a pair that was cut.
-template <typename T, int D>
-__global__ void __launch_bounds__(512) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
-    constexpr int LPR = D / 4;                                              // lanes per partial row
-    __shared__ float s_red[16];
-    __shared__ float4 s_o[512];
-    __shared__ float s_l[512 / LPR];
+// Merges the pieces of the pairs that were cut.  PARTS sets of D / 4 lanes share a row (one head of one pair), each taking
+// every PARTS-th piece, eight pieces' loads in flight at a time: the kernel is a chain of L2 latencies.  Many rows of a few
+// pieces: 1 set a row; few rows of many pieces: 256 / (D / 4) sets, and a CTA takes 64 of a row's dims only.
+template <typename T, int D, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? 256 : 128) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
+    constexpr int DIMS = WIDE ? 64 : D, LANES = DIMS / 4;
+    constexpr int PARTS = WIDE ? 256 / LANES : 1, ROWS = WIDE ? 1 : 128 / LANES;
+    __shared__ float4 s_o[WIDE ? PARTS : 1][LANES];
+    __shared__ float2 s_ml[WIDE ? PARTS : 1];
     pdl_wait();
     pdl_launch_dependents();
     const Split* split = reinterpret_cast<const Split*>(p.scratch);
-    const int b = blockIdx.y, hq = blockIdx.x, h = hq / p.group, head = hq - h * p.group;
-    const int share = split->share, c0 = split->cum[b];
-    const int groups = (split->cum[b + 1] - c0) / p.num_kv_heads;
-    if (groups == 0) return;
-    const int start = c0 + h * groups, first = start / share, last = (start + groups - 1) / share;
-    if (first == last) return;                                              // finished by its warp
-    const PartialView parts(p.scratch, 2 * (size_t)n_warps, p.group, D);
-    auto row_of = [&](int gw) -> int64_t {
-        return (2 * (int64_t)gw + (gw == first && start != first * share ? 1 : 0)) * p.group + head;
-    };
-    const int tid = threadIdx.x, nthr = blockDim.x;
-    float mx = kNoKey;
-    for (int i = first + tid; i <= last; i += nthr) mx = fmaxf(mx, parts.m[row_of(i)]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    if ((tid & 31) == 0) s_red[tid >> 5] = mx;
-    __syncthreads();
-    mx = s_red[0];
-    for (int i = 1; i < nthr / 32; i++) mx = fmaxf(mx, s_red[i]);
-
-    const int rp = tid / LPR, lanes = nthr / LPR, d4 = tid % LPR;
+    const int set = threadIdx.x / LANES, d4 = threadIdx.x % LANES;
+    const int hq = p.num_kv_heads * p.group;
+    const int row = WIDE ? blockIdx.x : blockIdx.x * ROWS + set, part = WIDE ? set : 0;
+    const bool live = row < p.n_seq * hq;
+    const int b = live ? row / hq : 0, h = (live ? row - b * hq : 0) / p.group, head = (live ? row - b * hq : 0) - h * p.group;
+    const int share = split->share, c0 = split->cum[b], c1 = split->cum[b + 1];
+    const int groups = (c1 - c0) / p.num_kv_heads, start = c0 + h * groups;
+    const int first = start / share, n = live && groups > 0 ? (start + groups - 1) / share - first + 1 : 0;
+    if (WIDE && n < 2) return;                                              // finished by its warp, or no keys
+    const Pieces pieces(p.scratch, n_warps, p.group, D);
+    const int64_t step = 2 * p.group, row1 = 2 * (int64_t)first * p.group + head;   // piece i > 0 at row1 + i * step
+    const int64_t row0 = row1 + (start != first * share ? p.group : 0);
+    const float* o = pieces.o + (WIDE ? blockIdx.y * DIMS : 0) + 4 * d4;
+    float m = kNoKey, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    if (n >= 2) {
+#pragma unroll 1
+        for (int i0 = part; i0 < n; i0 += 8 * PARTS) {
+            float2 ml[8];
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int i = min(i0 + k * PARTS, n - 1);
+                const int64_t r = i ? row1 + i * step : row0;
+                ml[k] = __ldcg(pieces.ml + r);
+                x[k] = __ldcg(reinterpret_cast<const float4*>(o + r * D));
+            }
+            float top = m;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, ml[k].x);
+            const float f0 = fast_exp2(m - top);
+            m = top;
+            l *= f0;
+            acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float f = i0 + k * PARTS < n ? fast_exp2(ml[k].x - top) : 0.f;
+                l += ml[k].y * f;
+                acc.x += x[k].x * f, acc.y += x[k].y * f, acc.z += x[k].z * f, acc.w += x[k].w * f;
+            }
+        }
+    }
+    if (WIDE) {
+        s_o[set][d4] = acc;
+        if (d4 == 0) s_ml[set] = make_float2(m, l);
+        __syncthreads();
+        if (set != 0) return;
+        float top = m;
+#pragma unroll 1
+        for (int i = 1; i < PARTS; i++) top = fmaxf(top, s_ml[i].x);
+        const float f0 = fast_exp2(m - top);
+        l *= f0;
+        acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
 #pragma unroll 4
-    for (int i = first + rp; i <= last; i += lanes) {
-        const int64_t r = row_of(i);
-        const float f = fast_exp2(parts.m[r] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(parts.o + r * D + 4 * d4);
-        sum += f * parts.l[r];
-        acc.x += f * x.x;
-        acc.y += f * x.y;
-        acc.z += f * x.z;
-        acc.w += f * x.w;
+        for (int i = 1; i < PARTS; i++) {
+            const float f = fast_exp2(s_ml[i].x - top);
+            const float4 x = s_o[i][d4];
+            l += s_ml[i].y * f;
+            acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
+        }
+    } else if (n < 2) {
+        return;
     }
-    s_o[tid] = acc;
-    if (d4 == 0) s_l[rp] = sum;
-    __syncthreads();
-    if (rp != 0) return;
-    sum = s_l[0];
-    for (int i = 1; i < lanes; i++) {
-        const float4 x = s_o[i * LPR + d4];
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-        sum += s_l[i];
-    }
-    if (!(sum != 0.f)) return;                                              // no visible key: the row stays as it is
-    const float inv = 1.f / sum;
+    if (!(l != 0.f)) return;                                                // no visible key: the row stays as it is
+    const float inv = 1.f / l;
     uint2 v;
     v.x = Elem<T>::pack2(acc.x * inv, acc.y * inv);
     v.y = Elem<T>::pack2(acc.z * inv, acc.w * inv);
-    T* dst = reinterpret_cast<T*>(p.out) + (((int64_t)b * p.num_kv_heads + h) * p.group + head) * D + 4 * d4;
-    *reinterpret_cast<uint2*>(dst) = v;
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (int64_t)row * D + (WIDE ? blockIdx.y * DIMS : 0) + 4 * d4) = v;
 }
 
 template <bool POOL8, typename T, int D, int NQ, bool LIST>
 cudaError_t launch_one(const AttendPagesParams& p, int num_sms, cudaStream_t stream) {
-    using R = Ring<POOL8, D>;
+    using R = Ring<POOL8, D, NQ>;
     constexpr int SLOT = 2 * 16 * D * (POOL8 ? 1 : 2) + (POOL8 ? 32 : 0);
     constexpr size_t ring = (size_t)R::kWarps * R::kStages * SLOT;
-    const size_t smem = ring + ((size_t)p.n_seq + 1) * sizeof(int);
+    const size_t smem = ring + (3 * (size_t)p.n_seq + 1) * sizeof(int);
     static std::atomic<bool> configured[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
         e = cudaFuncSetAttribute(attend_pages_kernel<POOL8, T, D, NQ, LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (int)(ring + (kMaxDecodeSeqs + 1) * sizeof(int)));
+                                 (int)(ring + (3 * kMaxPagesSeqs + 1) * sizeof(int)));
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
     }
     e = launch_pdl(attend_pages_kernel<POOL8, T, D, NQ, LIST>, dim3(num_sms), dim3(R::kWarps * 32), smem, stream, p);
     if (e != cudaSuccess) return e;
-    // many pieces a pair (few pairs): more threads share a row's merge
     const int n_warps = num_sms * R::kWarps;
-    const bool wide = (int64_t)p.n_seq * p.num_kv_heads * 16 < n_warps;
-    return launch_pdl(merge_pieces_kernel<T, D>, dim3(p.group * p.num_kv_heads, p.n_seq), dim3(wide ? 512 : 128), 0, stream, p, n_warps);
+    const int64_t pairs = (int64_t)p.n_seq * p.num_kv_heads, rows = pairs * p.group;
+    // about n_warps / pairs pieces a row
+    if (pairs * 8 < n_warps)
+        return launch_pdl(merge_pieces_kernel<T, D, true>, dim3((unsigned)rows, D / 64), dim3(256), 0, stream, p, n_warps);
+    constexpr int per_cta = 128 / (D / 4);
+    return launch_pdl(merge_pieces_kernel<T, D, false>, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(128), 0, stream, p, n_warps);
 }
 
 template <typename T, int D, int NQ>
@@ -635,13 +732,13 @@ cudaError_t launch_group(const AttendPagesParams& p, bool pool8, int num_sms, cu
 }  // namespace
 
 size_t attend_pages_scratch_bytes(int group, int head_dim, int num_sms) {
-    const size_t slots = 2 * (size_t)num_sms * 16;                          // at most 16 warps an SM
-    return (kSplitFloats + slots * group * (head_dim + 2)) * sizeof(float);
+    const size_t rows = 2 * (size_t)num_sms * 16 * group;                  // at most 16 warps a CTA
+    return (kSplitFloats + rows * (head_dim + 2)) * sizeof(float);
 }
 
 cudaError_t launch_attend_pages(const AttendPagesParams& p, bool pool8, int head_dim, int dtype, int num_sms, cudaStream_t stream) {
     if (p.n_seq <= 0 || p.max_kv_len <= 0) return cudaSuccess;
-    if (p.n_seq > kMaxDecodeSeqs || p.group < 1 || p.group > 16 || p.page_size % 16 != 0) return cudaErrorInvalidValue;
+    if (p.n_seq > kMaxPagesSeqs || p.group < 1 || p.group > 16 || p.page_size % 16 != 0) return cudaErrorInvalidValue;
     const bool f16 = dtype == DRKV_DTYPE_F16;
     switch (head_dim) {
         case 64: return f16 ? launch_group<__half, 64>(p, pool8, num_sms, stream) : launch_group<__nv_bfloat16, 64>(p, pool8, num_sms, stream);

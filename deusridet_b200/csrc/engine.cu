@@ -1137,9 +1137,9 @@ static int attend_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_r
     // the kernel counts 16-key groups of a launch in 32 bits
     int64_t groups = ((int64_t)max_kv_len + 15) / 16;
     if (d_list && (int64_t)list_len * (g.page_size / 16) < groups) groups = (int64_t)list_len * (g.page_size / 16);
-    const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxDecodeSeqs;
+    const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxPagesSeqs;
     if (cap < 1) return set_err(DRKV_ERR_CAPACITY, "attend: %d keys of %d KV heads are more than one launch takes", max_kv_len, g.num_kv_heads);
-    const int step = cap < kMaxDecodeSeqs ? (int)cap : kMaxDecodeSeqs;
+    const int step = cap < kMaxPagesSeqs ? (int)cap : kMaxPagesSeqs;
     const size_t row_bytes = (size_t)g.num_q_heads * g.head_dim * 2;
     for (int s0 = 0; s0 < n_seq; s0 += step) {
         p.n_seq = n_seq - s0 < step ? n_seq - s0 : step;

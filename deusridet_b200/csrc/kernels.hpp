@@ -199,9 +199,10 @@ struct AttendPagesParams {
     const void* q;            // [n_seq][Hq][D]
     void* out;
     float scale_log2;         // scale * log2(e)
-    float* scratch;           // partials and the work split, attend_pages_scratch_bytes
+    float* scratch;           // partials, attend_pages_scratch_bytes
     int* error_word;
 };
+constexpr int kMaxPagesSeqs = 1024;  // sequences of one launch (their lengths sit in shared memory)
 size_t attend_pages_scratch_bytes(int group, int head_dim, int num_sms);
 cudaError_t launch_attend_pages(const AttendPagesParams& p, bool pool8, int head_dim, int dtype, int num_sms, cudaStream_t stream);
 
