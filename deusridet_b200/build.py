@@ -16,7 +16,7 @@ LIB = os.path.join(HERE, "libdrkv.so")
 
 CUDA_SOURCES = ["engine.cu", "append.cu", "attend_decode.cu", "stateless.cu", "decode_noalloc.cu", "attend_prefill.cu", "gather_scatter.cu", "rope.cu", "cache8.cu", "attend_pages.cu", "page_bounds.cu"]
 CXX_SOURCES = ["page_book.cpp", "page_store.cpp", "sharding.cpp"]
-HEADERS = ["kernels.hpp", "kv_common.cuh", "page_book.hpp", "page_store.hpp", "exchange.cuh", "stateless.hpp", "device_guard.hpp", "sm100_primitives.cuh", os.path.join("..", "..", "include", "drkv.h")]
+HEADERS = ["kernels.hpp", "kv_common.cuh", "page_book.hpp", "page_store.hpp", "exchange.cuh", "stateless.hpp", "device_guard.hpp", "row_tiles.cuh", "sm100_primitives.cuh", os.path.join("..", "..", "include", "drkv.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

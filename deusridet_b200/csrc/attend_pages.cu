@@ -28,6 +28,7 @@
 
 #include "kernels.hpp"
 #include "kv_common.cuh"
+#include "row_tiles.cuh"
 #include "sm100_primitives.cuh"
 
 namespace drkv {
@@ -47,40 +48,6 @@ template <int NQ> struct Ring<false, 64, NQ>  { static constexpr int kWarps = 16
 template <int NQ> struct Ring<false, 128, NQ> { static constexpr int kWarps = 8, kStages = 3; };    // 192 KB
 template <int NQ> struct Ring<false, 256, NQ> { static constexpr int kWarps = 6, kStages = 2; };    // 192 KB
 
-// A tile is 16 rows of ROWB bytes in shared memory; chunks of 16 bytes are permuted so that both access patterns are free
-// of bank conflicts: rows (g) x chunks (t) for K, rows (2t) x chunks (g) for V, g = lane / 4, t = lane % 4.
-template <int ROWB>
-__device__ __forceinline__ uint32_t tile_off(int row, int chunk) {
-    if (ROWB == 64)                    // two rows share a 128-byte line
-        return (row >> 1) * 128 + (((((row & 1) << 2) | chunk) ^ (((row >> 1) & 3) << 1)) << 4);
-    return row * ROWB + ((chunk ^ ((((row >> 1) & 3) << 1) ^ ((row & 1) << 2))) << 4);
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint32_t lds8(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-// 16 bytes from global to shared memory; the second form writes zeros where !live
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -608,12 +575,13 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
     copies_wait<0>();
 }
 
-// Merges the pieces of the pairs that were cut.  PARTS sets of D / 4 lanes share a row (one head of one pair), each taking
-// every PARTS-th piece, eight pieces' loads in flight at a time: the kernel is a chain of L2 latencies.  Many rows of a few
-// pieces: 1 set a row; few rows of many pieces: 256 / (D / 4) sets, and a CTA takes 64 of a row's dims only.
-template <typename T, int D, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 256 : 128) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
-    constexpr int DIMS = WIDE ? 64 : D, LANES = DIMS / 4;
+// Merges the pieces of the pairs that were cut.  Sets of lanes share a row (one head of one pair), each taking every
+// PARTS-th piece, eight pieces' loads in flight at a time: the kernel is a chain of L2 latencies.  CTA_DIMS == 0: many rows of a
+// few pieces, one set a row.  CTA_DIMS > 0: a CTA takes that many of one row with as many sets as fit.
+template <typename T, int D, int CTA_DIMS>
+__global__ void __launch_bounds__(CTA_DIMS ? 256 : 128) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
+    constexpr bool WIDE = CTA_DIMS > 0;
+    constexpr int DIMS = WIDE ? CTA_DIMS : D, LANES = DIMS / 4;
     constexpr int PARTS = WIDE ? 256 / LANES : 1, ROWS = WIDE ? 1 : 128 / LANES;
     __shared__ float4 s_o[WIDE ? PARTS : 1][LANES];
     __shared__ float2 s_ml[WIDE ? PARTS : 1];
@@ -642,10 +610,14 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128) merge_pieces_kernel(const At
             float4 x[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const int i = min(i0 + k * PARTS, n - 1);
+                const int i = i0 + k * PARTS;
                 const int64_t r = i ? row1 + i * step : row0;
-                ml[k] = __ldcg(pieces.ml + r);
-                x[k] = __ldcg(reinterpret_cast<const float4*>(o + r * D));
+                ml[k] = make_float2(kNoKey, 0.f);
+                x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (i < n) {
+                    ml[k] = __ldcg(pieces.ml + r);
+                    x[k] = __ldcg(reinterpret_cast<const float4*>(o + r * D));
+                }
             }
             float top = m;
 #pragma unroll
@@ -656,7 +628,7 @@ __global__ void __launch_bounds__(WIDE ? 256 : 128) merge_pieces_kernel(const At
             acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float f = i0 + k * PARTS < n ? fast_exp2(ml[k].x - top) : 0.f;
+                const float f = fast_exp2(ml[k].x - top);                   // absent: 2^(no key - top) * 0
                 l += ml[k].y * f;
                 acc.x += x[k].x * f, acc.y += x[k].y * f, acc.z += x[k].z * f, acc.w += x[k].w * f;
             }
@@ -711,11 +683,13 @@ cudaError_t launch_one(const AttendPagesParams& p, int num_sms, cudaStream_t str
     if (e != cudaSuccess) return e;
     const int n_warps = num_sms * R::kWarps;
     const int64_t pairs = (int64_t)p.n_seq * p.num_kv_heads, rows = pairs * p.group;
-    // about n_warps / pairs pieces a row
-    if (pairs * 8 < n_warps)
-        return launch_pdl(merge_pieces_kernel<T, D, true>, dim3((unsigned)rows, D / 64), dim3(256), 0, stream, p, n_warps);
+    // about n_warps / pairs pieces a row; few rows are spread over CTAs of 32 dims (32 rows of 296 pieces: 8 us against 9,
+    // 512 rows of 37 pieces: 19 us against 7 by whole rows)
+    if (rows * (D / 32) <= 2 * num_sms)
+        return launch_pdl(merge_pieces_kernel<T, D, 32>, dim3((unsigned)rows, D / 32), dim3(256), 0, stream, p, n_warps);
+    if (pairs * 8 < n_warps) return launch_pdl(merge_pieces_kernel<T, D, D>, dim3((unsigned)rows), dim3(256), 0, stream, p, n_warps);
     constexpr int per_cta = 128 / (D / 4);
-    return launch_pdl(merge_pieces_kernel<T, D, false>, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(128), 0, stream, p, n_warps);
+    return launch_pdl(merge_pieces_kernel<T, D, 0>, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(128), 0, stream, p, n_warps);
 }
 
 template <typename T, int D, int NQ>

@@ -10,33 +10,48 @@
 // 16-byte vectors on the 16-bit side and 8-byte ones on the 8-bit side, maxima by warp shuffle.
 #include "kernels.hpp"
 #include "kv_common.cuh"
+#include "sm100_primitives.cuh"
 
 namespace drkv {
 
 namespace {
 
 constexpr int kThreads8 = 256;
-constexpr int kMaxPairs8 = 128;   // rotary_dim / 2 <= head_dim / 2
+constexpr int kMaxTokens8 = 32;   // tokens of one CTA of the append
+constexpr int kBatch8 = 4;        // rows a lane has in flight
 
-// Quantises the row of which each of its LANES lanes holds 8 elements; writes bytes and exponent where store is true.
+// n / d for n * d < 2^32 by a multiplication; magic 0 stands for d = 1.
+__host__ __device__ __forceinline__ uint32_t magic_of(uint32_t d) { return d <= 1 ? 0 : (uint32_t)((0x100000000ull + d - 1) / d); }
+__device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t magic) { return magic ? __umulhi(n, magic) : n; }
+
+// Quantises the row of which each of its LANES lanes holds 8 elements; row: its index in the block's rows (K plane, then V
+// plane, exponents in the same order).
 template <int LANES>
-__device__ __forceinline__ void quantise_row(const float (&x)[8], uint8_t* dst, uint8_t* dst_exp, int l, bool store) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
-        amax = max(amax, a < 0x7f800000u ? a : 0u);
-    }
+__device__ __forceinline__ void quantise_row(const float (&x)[8], uint8_t* block, int64_t exponents, int row, int l, bool store) {
+    // the maximum of |x|; NaN is passed over by the maximum, an infinity makes the row look again
+    float top = fmax3(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3]));
+    top = fmax3(fmax3(top, fabsf(x[4]), fabsf(x[5])), fabsf(x[6]), fabsf(x[7]));
+    uint32_t amax = __float_as_uint(top == top ? top : 0.f);
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (__any_sync(0xffffffffu, amax >= 0x7f800000u)) {
+        amax = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
+            amax = max(amax, a < 0x7f800000u ? a : 0u);
+        }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    }
     const int e = e4m3_row_exponent(amax);
     const float inv = exp2_int(-e);
     uint2 v;
-    v.x = f32x2_to_e4m3x2(x[0] * inv, x[1] * inv) | f32x2_to_e4m3x2(x[2] * inv, x[3] * inv) << 16;
-    v.y = f32x2_to_e4m3x2(x[4] * inv, x[5] * inv) | f32x2_to_e4m3x2(x[6] * inv, x[7] * inv) << 16;
+    v.x = f32x4_to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+    v.y = f32x4_to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
     if (store) {
-        *reinterpret_cast<uint2*>(dst + 8 * l) = v;
-        if (l == 0) *dst_exp = (uint8_t)(e + 127);
+        *reinterpret_cast<uint2*>(block + (int64_t)row * (8 * LANES) + 8 * l) = v;
+        if (l == 0) block[exponents + row] = (uint8_t)(e + 127);
     }
 }
 
@@ -54,15 +69,28 @@ __device__ __forceinline__ void unpack8(const Vec16& v, float (&x)[8]) {
 // row above 64 512 may have rounded up past the largest value and reads as that, and a rotated row's elements may lie
 // between the type's steps of 2^-24 and are rounded to the nearest.
 template <typename T>
-__device__ __forceinline__ Vec16 expand8(uint2 q, float scale) {
+__device__ __forceinline__ Vec16 expand8(uint2 q, int exp_byte) {
+    const int e = exp_byte - 127;
+    uint32_t h[4];
+    e4m3x4_to_f16x4(q.x, h[0], h[1]);
+    e4m3x4_to_f16x4(q.y, h[2], h[3]);
     Vec16 v;
+    if (Elem<T>::kUmmaFormat == 0 && e >= -14 && e <= 7) {           // within fp16's normal powers and below its end
+        const __half2 scale = __half2half2(__ushort_as_half((unsigned short)((e + 15) << 10)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), scale);
+            v.w[i] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        return v;
+    }
+    const float scale = exp2_int(e);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t two = ((i & 2) ? q.y : q.x) >> (16 * (i & 1));
-        const float2 f = Elem<__half>::unpack2(e4m3x2_to_f16x2(two & 0xffffu));
+        const float2 f = Elem<__half>::unpack2(h[i]);
         float a = f.x * scale, b = f.y * scale;
         if (Elem<T>::kUmmaFormat == 0) {
-            a = fabsf(a) > 65504.f ? copysignf(65504.f, a) : a;   // NaN compares false
+            a = fabsf(a) > 65504.f ? copysignf(65504.f, a) : a;      // NaN compares false
             b = fabsf(b) > 65504.f ? copysignf(65504.f, b) : b;
         }
         v.w[i] = Elem<T>::pack2(a, b);
@@ -70,93 +98,149 @@ __device__ __forceinline__ Vec16 expand8(uint2 q, float scale) {
     return v;
 }
 
-// One CTA per token: D / 8 lanes per row, K heads first, then V heads.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads8) append8_kernel(const Append8Params p) {
+// Where a CTA's tokens lie: block start (bytes; < 0: hole or no position) and slot.
+struct TokenPlace {
+    int64_t block;
+    int slot, pos;
+};
+
+// A CTA takes some tokens, D / 8 lanes per row: a token's K heads, then its V heads, as in its page block.  BATCH rows a lane
+// are read before the first is worked on (a row at a time, one token per CTA: 30 000 tokens of 4 heads of 256 took 77 us).
+template <typename T, int D, int BATCH>
+__global__ void __launch_bounds__(kThreads8) append8_kernel(const Append8Params p, int n_all, int tokens_per_cta, uint32_t magic_rows) {
     constexpr int LANES = D / 8, ROWS = kThreads8 / LANES;
-    __shared__ float s_cos[kMaxPairs8], s_sin[kMaxPairs8];
+    extern __shared__ float s_trig[];                                // [token][2][half]
+    __shared__ TokenPlace s_place[kMaxTokens8];
     pdl_wait();
     pdl_launch_dependents();
-    const int tok = blockIdx.x;
-    int row = p.row, pos = p.pos_start + tok;
-    if (p.rows != nullptr) {
-        row = __ldg(p.rows + tok);
-        pos = __ldg(p.pos + tok) + p.pos_start;                      // -1 where the lengths count the new token
-    }
+    const int tok0 = blockIdx.x * tokens_per_cta, n_tok = min(tokens_per_cta, n_all - tok0);
     const int P = p.layout.page_size, H = p.layout.num_kv_heads;
-    const int logical = pos >= 0 ? pos / P : 0, slot = pos - logical * P;
-    int page = -1;
-    if (pos >= 0 && logical < p.table_stride && row >= 0 && row < p.max_rows)
-        page = __ldg(p.tables + (int64_t)row * p.table_stride + logical);
-    if (page < 0 || page >= p.layout.max_pages) return;             // hole or no position: nothing to write into
-    const int half = p.rotary_dim >> 1;
-    for (int i = threadIdx.x; i < half; i += kThreads8)              // the angles of append_rope_kernel, bit for bit
-        sincos_det(__fmul_rn((float)pos, __ldg(p.inv_freq + i)), s_sin[i], s_cos[i]);
-    if (half > 0) __syncthreads();
-    const int l = threadIdx.x % LANES;
-    uint8_t* block = p.pool + p.layout.block_of(p.layer, page);
-    for (int r0 = 0; r0 < 2 * H; r0 += ROWS) {
-        const int r = r0 + threadIdx.x / LANES;
-        const bool live = r < 2 * H;
-        const int kv = r >= H, h = kv ? r - H : r;
-        float x[8] = {};
-        if (live) {
-            const T* src = reinterpret_cast<const T*>(kv ? p.v_src : p.k_src) + ((int64_t)tok * H + h) * D;
-            unpack8<T>(ldg16(src + 8 * l), x);
-        }
-        if (half > 0) {
-            const int hl = half / 8;                                 // lanes of one rotated half (rotary_dim % 16 == 0)
-            const bool first = l < hl, second = l >= hl && l < 2 * hl;
-            // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
-            const int base = (threadIdx.x & 31) - l, other = base + (first ? l + hl : second ? l - hl : l);
+    const int l = threadIdx.x % LANES, total = n_tok * 2 * H;
+    const int64_t exponents = 2 * p.layout.plane;
+    Vec16 in[BATCH];
+    auto read = [&](int r0) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float o = __shfl_sync(0xffffffffu, x[i], other);
-                if (!kv && (first || second)) {
-                    const int j = 8 * (first ? l : l - hl) + i;
-                    float y0, y1;
-                    rope_pair(first ? x[i] : o, first ? o : x[i], s_cos[j], s_sin[j], y0, y1);
-                    x[i] = first ? y0 : y1;
-                }
+        for (int u = 0; u < BATCH; u++) {
+            const int r = r0 + u * ROWS;
+            in[u] = Vec16{{0u, 0u, 0u, 0u}};
+            if (r < total) {
+                const int t = div_magic(r, magic_rows), kh = r - t * 2 * H;
+                const T* src = reinterpret_cast<const T*>(kh < H ? p.k_src : p.v_src) + ((int64_t)(tok0 + t) * H + (kh < H ? kh : kh - H)) * D;
+                in[u] = ldg16(src + 8 * l);
             }
         }
-        quantise_row<LANES>(x, block + p.layout.row(kv, h, slot), block + p.layout.exponent(kv, h, slot), l, live);
+    };
+    read(threadIdx.x / LANES);                                       // on their way while the places are worked out
+    if (threadIdx.x < n_tok) {
+        const int tok = tok0 + threadIdx.x;
+        int row = p.row, pos = p.pos_start + tok;
+        if (p.rows != nullptr) {
+            row = __ldg(p.rows + tok);
+            pos = __ldg(p.pos + tok) + p.pos_start;                  // -1 where the lengths count the new token
+        }
+        const int logical = pos >= 0 ? pos / P : 0;
+        int page = -1;
+        if (pos >= 0 && logical < p.table_stride && row >= 0 && row < p.max_rows)
+            page = __ldg(p.tables + (int64_t)row * p.table_stride + logical);
+        const bool live = page >= 0 && page < p.layout.max_pages;    // hole or no position: nothing to write into
+        s_place[threadIdx.x] = TokenPlace{live ? p.layout.block_of(p.layer, page) : -1, pos - logical * P, pos};
+    }
+    __syncthreads();
+    const int half = p.rotary_dim >> 1;
+    if (half > 0) {
+        for (int i = threadIdx.x; i < n_tok * half; i += kThreads8) {   // the angles of append_rope_kernel, bit for bit
+            const int t = i / half, j = i - t * half;
+            sincos_det(__fmul_rn((float)s_place[t].pos, __ldg(p.inv_freq + j)), s_trig[(2 * t + 1) * half + j], s_trig[2 * t * half + j]);
+        }
+        __syncthreads();
+    }
+    for (int r0 = threadIdx.x / LANES; r0 < total + threadIdx.x / LANES; r0 += BATCH * ROWS) {   // the whole CTA together
+#pragma unroll
+        for (int u = 0; u < BATCH; u++) {
+            const int r = r0 + u * ROWS;
+            const int t = div_magic(min(r, total - 1), magic_rows), kh = min(r, total - 1) - t * 2 * H;
+            float x[8];
+            unpack8<T>(in[u], x);
+            if (half > 0) {
+                const int hl = half / 8;                             // lanes of one rotated half (rotary_dim % 16 == 0)
+                const bool first = l < hl, second = l >= hl && l < 2 * hl;
+                // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
+                const int base = (threadIdx.x & 31) - l, other = base + (first ? l + hl : second ? l - hl : l);
+                const float* c = s_trig + 2 * t * half + 8 * (first ? l : second ? l - hl : 0);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float o = __shfl_sync(0xffffffffu, x[i], other);
+                    if (kh < H && (first || second)) {
+                        float y0, y1;
+                        rope_pair(first ? x[i] : o, first ? o : x[i], c[i], c[half + i], y0, y1);
+                        x[i] = first ? y0 : y1;
+                    }
+                }
+            }
+            const TokenPlace at = s_place[t];
+            quantise_row<LANES>(x, p.pool + at.block, exponents, kh * P + at.slot, l, r < total && at.block >= 0);
+        }
+        read(r0 + BATCH * ROWS);
     }
 }
 
-// grid (token blocks, layer * 2 + plane): a CTA takes kFlatTokens tokens of one plane.
+// grid (token blocks, layer * 2 + plane): a CTA takes kFlatTokens tokens of one plane, four rows a lane at a time.
 constexpr int kFlatTokens = 16;
 template <typename T, int D, bool TO_FLAT>
-__global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params p) {
+__global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params p, uint32_t magic_heads) {
     constexpr int LANES = D / 8, ROWS = kThreads8 / LANES;
+    __shared__ TokenPlace s_place[kFlatTokens];
     pdl_wait();
     pdl_launch_dependents();
     const int H = p.layout.num_kv_heads, P = p.layout.page_size;
     const int layer = blockIdx.y >> 1, kv = blockIdx.y & 1;
     const int tok0 = blockIdx.x * kFlatTokens, n_tok = min(kFlatTokens, p.num_tokens - tok0);
-    const int l = threadIdx.x % LANES;
-    T* flat = reinterpret_cast<T*>(p.flat) + ((int64_t)blockIdx.y * p.num_tokens + tok0) * H * D;
-#pragma unroll 4
-    for (int r0 = 0; r0 < n_tok * H; r0 += ROWS) {
-        const int r = r0 + threadIdx.x / LANES;
-        const bool live = r < n_tok * H;
-        const int t = live ? r / H : 0, h = live ? r - t * H : 0;
-        const int pos = p.start_token + tok0 + t, logical = pos / P, slot = pos - logical * P;
-        int page = logical < p.table_stride ? __ldg(p.table + logical) : -1;
-        if (page >= p.layout.max_pages) page = -1;
-        uint8_t* block = p.pool + (page < 0 ? 0 : p.layout.block_of(layer, page));
-        uint8_t* row = block + p.layout.row(kv, h, slot);
-        uint8_t* exponent = block + p.layout.exponent(kv, h, slot);
-        T* f = flat + (int64_t)r * D + 8 * l;
-        if (TO_FLAT) {
-            if (!live) continue;
-            Vec16 v = Vec16{{0u, 0u, 0u, 0u}};                       // a hole reads as zeros
-            if (page >= 0) v = expand8<T>(*reinterpret_cast<const uint2*>(row + 8 * l), exp2_int((int)*exponent - 127));
-            stg16(f, v);
-        } else {
-            float x[8] = {};
-            if (live) unpack8<T>(ldg16(f), x);
-            quantise_row<LANES>(x, row, exponent, l, live && page >= 0);
+    if (threadIdx.x < n_tok) {
+        const int pos = p.start_token + tok0 + threadIdx.x, logical = pos / P;
+        const int page = logical < p.table_stride ? __ldg(p.table + logical) : -1;
+        const bool live = page >= 0 && page < p.layout.max_pages;
+        s_place[threadIdx.x] = TokenPlace{live ? p.layout.block_of(layer, page) : -1, pos - logical * P, pos};
+    }
+    __syncthreads();
+    const int l = threadIdx.x % LANES, total = n_tok * H;
+    const int64_t exponents = 2 * p.layout.plane;
+    T* flat = reinterpret_cast<T*>(p.flat) + ((int64_t)blockIdx.y * p.num_tokens + tok0) * H * D + 8 * l;
+    for (int r0 = threadIdx.x / LANES; r0 < total + threadIdx.x / LANES; r0 += kBatch8 * ROWS) {   // the whole CTA together
+        uint2 q[kBatch8];
+        uint8_t e[kBatch8];
+        Vec16 in[kBatch8];
+#pragma unroll
+        for (int u = 0; u < kBatch8; u++) {
+            const int r = r0 + u * ROWS;
+            q[u] = make_uint2(0u, 0u);
+            e[u] = 0;
+            in[u] = Vec16{{0u, 0u, 0u, 0u}};
+            if (r >= total) continue;
+            if (TO_FLAT) {
+                const int t = div_magic(r, magic_heads), h = r - t * H;
+                const TokenPlace at = s_place[t];
+                if (at.block >= 0) {                                 // a hole reads as zeros
+                    const uint8_t* block = p.pool + at.block;
+                    const int row = (kv * H + h) * P + at.slot;
+                    q[u] = __ldcs(reinterpret_cast<const uint2*>(block + (int64_t)row * D) + l);
+                    e[u] = block[exponents + row];
+                }
+            } else {
+                in[u] = ldg16(flat + (int64_t)r * D);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch8; u++) {
+            const int r = r0 + u * ROWS;
+            if (TO_FLAT) {
+                if (r < total) stg16(flat + (int64_t)r * D, expand8<T>(q[u], e[u]));
+            } else {
+                const int t = div_magic(min(r, total - 1), magic_heads), h = min(r, total - 1) - t * H;
+                const TokenPlace at = s_place[t];
+                float x[8];
+                unpack8<T>(in[u], x);
+                quantise_row<LANES>(x, p.pool + at.block, exponents, (kv * H + h) * P + at.slot, l, r < total && at.block >= 0);
+            }
         }
     }
 }
@@ -184,13 +268,25 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
     const uint8_t* block = p.pool + p.layout.block_of(p.layer, page);
     const uint8_t* exps = block + 2 * p.layout.plane;
     T* image = reinterpret_cast<T*>(p.image) + (int64_t)page * rows * D;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < rows * LANES; i += kThreads8) {
-        const int r = i / LANES;
-        Vec16 v = Vec16{{0u, 0u, 0u, 0u}};
-        if (r % P < visible)
-            v = expand8<T>(__ldg(reinterpret_cast<const uint2*>(block) + i), exp2_int((int)__ldg(exps + r) - 127));
-        stg16(image + (int64_t)i * 8, v);
+    const int total = rows * LANES;                                  // a multiple of 4 x 256 elements of 8 is the rule, not a must
+    for (int i0 = threadIdx.x; i0 < total; i0 += kBatch8 * kThreads8) {
+        uint2 q[kBatch8];
+        uint8_t e[kBatch8];
+#pragma unroll
+        for (int u = 0; u < kBatch8; u++) {
+            const int i = i0 + u * kThreads8, r = i / LANES;
+            q[u] = make_uint2(0u, 0u);
+            e[u] = 0;
+            if (i < total && (visible == P || r % P < visible)) {
+                q[u] = __ldcs(reinterpret_cast<const uint2*>(block) + i);
+                e[u] = __ldg(exps + r);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch8; u++) {
+            const int i = i0 + u * kThreads8;
+            if (i < total) stg16(image + (int64_t)i * 8, expand8<T>(q[u], e[u]));
+        }
     }
 }
 
@@ -217,19 +313,29 @@ cudaError_t by_shape(const P& p, int dtype, int head_dim, int n, cudaStream_t st
 template <typename T, int D>
 struct AppendLaunch {
     static cudaError_t run(const Append8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(append8_kernel<T, D>, dim3(n), dim3(kThreads8), 0, s, p);
+        // one row a lane and one token a CTA for decode batches; four rows a lane, and the tokens for them, once such CTAs
+        // fill the SMs twice over (4 of 256 threads each)
+        constexpr int ROWS = kThreads8 / (D / 8);
+        const int H = p.layout.num_kv_heads;
+        int per = 1;
+        while (per < kMaxTokens8 && per * 2 * H < 4 * ROWS) per *= 2;
+        const uint32_t magic = magic_of(2 * H);
+        if (n < per * 4 * 2 * 148)
+            return launch_pdl(append8_kernel<T, D, 1>, dim3(n), dim3(kThreads8), p.rotary_dim * sizeof(float), s, p, n, 1, magic);
+        return launch_pdl(append8_kernel<T, D, 4>, dim3((n + per - 1) / per), dim3(kThreads8), (size_t)per * p.rotary_dim * sizeof(float),
+                          s, p, n, per, magic);
     }
 };
 template <typename T, int D>
 struct ExtractLaunch {
     static cudaError_t run(const Flat8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(flat_copy8_kernel<T, D, true>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p);
+        return launch_pdl(flat_copy8_kernel<T, D, true>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p, magic_of(p.layout.num_kv_heads));
     }
 };
 template <typename T, int D>
 struct InjectLaunch {
     static cudaError_t run(const Flat8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(flat_copy8_kernel<T, D, false>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p);
+        return launch_pdl(flat_copy8_kernel<T, D, false>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p, magic_of(p.layout.num_kv_heads));
     }
 };
 template <typename T, int D>

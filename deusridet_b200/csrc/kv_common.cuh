@@ -79,10 +79,11 @@ __device__ __forceinline__ void e4m3x4_to_f16x4(uint32_t four_bytes, uint32_t& l
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(lo), "=r"(hi) : "r"(four_bytes));
 }
-// bytes: lo in the lower one.  Values beyond 448 and infinities become 448, NaN stays NaN.
-__device__ __forceinline__ uint32_t f32x2_to_e4m3x2(float lo, float hi) {
+// bytes in order, a the lowest.  Values beyond 448 and infinities become 448, NaN stays NaN.
+__device__ __forceinline__ uint32_t f32x4_to_e4m3x4(float a, float b, float c, float d) {
     uint32_t r;
-    asm("{\n\t.reg .b16 h;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %2, %1;\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(r) : "f"(lo), "f"(hi));
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
 

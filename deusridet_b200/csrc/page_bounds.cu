@@ -15,6 +15,8 @@
 
 #include "kernels.hpp"
 #include "kv_common.cuh"
+#include "row_tiles.cuh"
+#include "sm100_primitives.cuh"
 
 namespace drkv {
 
@@ -187,48 +189,101 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One warp per 8 pages at a time of one (sequence, KV head): the pages are the columns of the int8 tiles, the group's heads
-// the rows.  A lane takes whole 16-byte chunks of a page's 2 D bound bytes (contraction order is free) straight from
-// global memory into operand registers; the query bytes stay in registers over all pages of the warp.
-// grid (page blocks, KV heads, sequences); keys[(seq * Hkv + head) * stride + page].
-constexpr int kScoreWarps = 4;
+// One warp walks pages of one (sequence, KV head), 8 to an int8 tile: the pages are its columns, the group's heads its rows.
+// Contraction order is free: a lane takes whole 16-byte chunks of a page's 2 D bound bytes, and the query bytes of the same
+// dims stay in registers over all pages.  The pass is bound by bytes in flight: bounds come by cp.async into a ring per warp,
+// 4 KB a stage, three stages ahead (held in registers, 4 to 8 KB a warp, 42 000 pages of 8 heads took 27-33 us).
+// The warps of a CTA take neighbouring heads of the same pages (their bounds lie side by side in memory), and where there
+// are fewer than four, stretches of the pages.  grid (page blocks, KV heads / heads_per_cta, sequences);
+// keys[(seq * Hkv + head) * stride + page].
+constexpr int kScoreWarps = 4, kScoreStages = 4, kScoreStageBytes = 4096;
 template <typename T, int D, bool HI>
-__global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const SelectParams p, int pages_per_cta) {
+__global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const SelectParams p, int pages_per_cta, int heads_per_cta) {
     constexpr int CH = D / 64;                                              // query chunks (16 dims) a lane owns
-    pdl_wait();
-    pdl_launch_dependents();
-    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    constexpr int ROWB = 2 * D, CPR = ROWB / 16, SP = kScoreStageBytes / ROWB, TILES = SP / 8;   // pages and tiles of a stage
+    constexpr int NR = HI ? 2 : 1;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int b = blockIdx.z, lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y * heads_per_cta + w % heads_per_cta, part = w / heads_per_cta, parts = kScoreWarps / heads_per_cta;
+    // lengths, rows, tables and bounds come from further back than the kernel directly in front, or from this library's
     const int row = __ldg(p.rows + b);
     const int len = min(__ldg(p.kv_len + b), p.max_kv_len);
-    if (len <= 0 || row < 0 || row >= p.max_rows) return;
-    const int n = min((len - 1) / p.page_size + 1, p.table_stride);
-    const int first = blockIdx.x * pages_per_cta, last = min(n, first + pages_per_cta);
-    if (first >= last) return;
-    // ---- query bytes ----
-    uint32_t up[HI ? 2 : 1][CH][4], down[HI ? 2 : 1][CH][4];
-    int f[HI ? 2 : 1];
+    const int n = len <= 0 || row < 0 || row >= p.max_rows ? 0 : min((len - 1) / p.page_size + 1, p.table_stride);
+    const int per_part = pages_per_cta / parts;                             // a multiple of 32
+    const int begin = blockIdx.x * pages_per_cta + part * per_part, last = min(n, begin + per_part);
+    const int32_t* table = p.tables + (int64_t)row * p.table_stride;
+    auto page_ids = [&](int i) -> int {                                     // lane i: page i of a window of 32
+        return i + lane < last ? __ldg(table + i + lane) : -1;
+    };
+    int iss32 = -1, iss_next = -1;
+    if (begin < last) {
+        iss32 = page_ids(begin);
+        iss_next = page_ids(begin + 32);
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    if (begin >= last) return;
+    const int64_t layer0 = (int64_t)p.layer * p.max_pages;
+    auto checked = [&](int page) -> int {
+        if (page >= p.max_pages) {
+            atomicExch(p.error_word, (int)KERR_BAD_PAGE);
+            return -1;
+        }
+        return page;
+    };
+    auto exponent_of = [&](int page) -> int { return page >= 0 ? __ldg(p.exponents + (layer0 + page) * p.num_kv_heads + h) : 0; };
+    iss32 = checked(iss32);
+    int page32 = iss32, next32 = checked(iss_next);                         // of the window being scored, and the one behind it
+    int e32 = exponent_of(page32), next_e = exponent_of(next32);
+    const uint32_t ring = smem_u32(smem) + w * kScoreStages * kScoreStageBytes;
+    const int n_stages = (last - begin + SP - 1) / SP;
+    auto issue = [&](int s) {
+        const int in_window = s * SP & 31;
+        if (in_window == 0 && s > 0) {
+            iss32 = checked(iss_next);
+            iss_next = page_ids(begin + s * SP + 32);
+        }
 #pragma unroll
-    for (int r = 0; r < (HI ? 2 : 1); r++) {
-        const int head = g + 8 * r;
-        const bool live = head < p.group;
-        const T* q = reinterpret_cast<const T*>(p.q) + (((int64_t)b * p.num_kv_heads + h) * p.group + head) * D;
+        for (int j = 0; j < SP * CPR / 32; j++) {
+            const int c = lane + 32 * j, r = c / CPR, chunk = c % CPR;
+            const int page = __shfl_sync(FULL, iss32, in_window + r);       // the bounds of a hole are not read
+            copy16_or_zero(ring + (s % kScoreStages) * kScoreStageBytes + tile_off<ROWB>(r, chunk),
+                           p.bounds + ((layer0 + max(page, 0)) * p.num_kv_heads + h) * ROWB + 16 * chunk, page >= 0);
+        }
+    };
+    // ---- query rows, then the first bounds, then the query bytes ----
+    uint32_t up[NR][CH][4], down[NR][CH][4];
+    int f[NR];
+    Vec16 raw[NR][CH][2];
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int i = 0; i < CH; i++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                raw[r][i][c] = Vec16{{0u, 0u, 0u, 0u}};
+                if (g + 8 * r < p.group)
+                    raw[r][i][c] = ldg16(reinterpret_cast<const T*>(p.q) + (((int64_t)b * p.num_kv_heads + h) * p.group + g + 8 * r) * D + 16 * (t + 4 * i) + 8 * c);
+            }
+#pragma unroll
+    for (int s = 0; s < kScoreStages - 1; s++) {
+        if (s < n_stages) issue(s);
+        copies_commit();
+    }
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
         float x[CH][16];
         uint32_t amax = 0;
 #pragma unroll
         for (int i = 0; i < CH; i++)
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                Vec16 v = Vec16{{0u, 0u, 0u, 0u}};
-                if (live) v = ldg16(q + 16 * (t + 4 * i) + 8 * c);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float2 y = Elem<T>::unpack2(v.w[j]);
-                    x[i][8 * c + 2 * j] = y.x;
-                    x[i][8 * c + 2 * j + 1] = y.y;
-                    // NaN counts as nothing, here and below
-                    amax = max(amax, y.x == y.x ? __float_as_uint(y.x) & 0x7fffffffu : 0u);
-                    amax = max(amax, y.y == y.y ? __float_as_uint(y.y) & 0x7fffffffu : 0u);
-                }
+            for (int j = 0; j < 8; j++) {
+                const float2 y = Elem<T>::unpack2(raw[r][i][j >> 2].w[j & 3]);
+                x[i][2 * j] = y.x;
+                x[i][2 * j + 1] = y.y;
+                // NaN counts as nothing, here and below
+                amax = max(amax, y.x == y.x ? __float_as_uint(y.x) & 0x7fffffffu : 0u);
+                amax = max(amax, y.y == y.y ? __float_as_uint(y.y) & 0x7fffffffu : 0u);
             }
         amax = max(amax, __shfl_xor_sync(FULL, amax, 1));
         amax = max(amax, __shfl_xor_sync(FULL, amax, 2));
@@ -250,64 +305,70 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
                 down[r][i][k] = d;
             }
     }
-    const int32_t* table = p.tables + (int64_t)row * p.table_stride;
     uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + h) * p.key_stride;
-    const int64_t layer0 = (int64_t)p.layer * p.max_pages;
-#pragma unroll 2
-    for (int p0 = first + 8 * w; p0 < last; p0 += 8 * kScoreWarps) {
-        // lane's page is p0 + g; the bounds of a hole are not read
-        int page = -1;
-        if (p0 + g < last) page = __ldg(table + p0 + g);
-        if (page >= p.max_pages) {
-            atomicExch(p.error_word, (int)KERR_BAD_PAGE);
-            page = -1;
-        }
-        const int64_t at = (layer0 + (page < 0 ? 0 : page)) * p.num_kv_heads + h;
-        const int8_t* bounds = p.bounds + at * 2 * D;
-        Vec16 v[2 * CH];
+    uint32_t key = kKeyHole;                                                // of this lane's page of the window
+    for (int s = 0; s < n_stages; s++) {
+        if (s + kScoreStages - 1 < n_stages) issue(s + kScoreStages - 1);
+        copies_commit();
+        copies_wait<kScoreStages - 1>();
+        __syncwarp();
+        const uint32_t stage = ring + (s % kScoreStages) * kScoreStageBytes;
+        const int in_window = s * SP & 31;
 #pragma unroll
-        for (int i = 0; i < 2 * CH; i++) {
-            v[i] = Vec16{{0u, 0u, 0u, 0u}};
-            if (page >= 0) v[i] = ldg16(bounds + 16 * (t + 4 * i));
-        }
-        const int e_own = page >= 0 ? p.exponents[at] : 0;
-        int acc[4] = {0, 0, 0, 0};
+        for (int k = 0; k < TILES; k++) {
+            int acc[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < CH; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k += 2) {
-                mma_s8(acc, up[0][i][k], HI ? up[HI ? 1 : 0][i][k] : 0u, up[0][i][k + 1], HI ? up[HI ? 1 : 0][i][k + 1] : 0u,
-                       v[i].w[k], v[i].w[k + 1]);
-                mma_s8(acc, down[0][i][k], HI ? down[HI ? 1 : 0][i][k] : 0u, down[0][i][k + 1], HI ? down[HI ? 1 : 0][i][k + 1] : 0u,
-                       v[CH + i].w[k], v[CH + i].w[k + 1]);
+            for (int i = 0; i < CH; i++) {
+                const uint4 hi4 = lds128(stage + tile_off<ROWB>(8 * k + g, t + 4 * i)), lo4 = lds128(stage + tile_off<ROWB>(8 * k + g, t + 4 * (CH + i)));
+                mma_s8(acc, up[0][i][0], HI ? up[NR - 1][i][0] : 0u, up[0][i][1], HI ? up[NR - 1][i][1] : 0u, hi4.x, hi4.y);
+                mma_s8(acc, up[0][i][2], HI ? up[NR - 1][i][2] : 0u, up[0][i][3], HI ? up[NR - 1][i][3] : 0u, hi4.z, hi4.w);
+                mma_s8(acc, down[0][i][0], HI ? down[NR - 1][i][0] : 0u, down[0][i][1], HI ? down[NR - 1][i][1] : 0u, lo4.x, lo4.y);
+                mma_s8(acc, down[0][i][2], HI ? down[NR - 1][i][2] : 0u, down[0][i][3], HI ? down[NR - 1][i][3] : 0u, lo4.z, lo4.w);
             }
-        // heads g (and g + 8), pages p0 + 2t and p0 + 2t + 1
+            // heads g (and g + 8), pages in_window + 8 k + 2 t + c of the window
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            const int e = __shfl_sync(FULL, e_own, 4 * (2 * t + c));
-            float best = -INFINITY;
+            for (int c = 0; c < 2; c++) {
+                const int e = __shfl_sync(FULL, e32, in_window + 8 * k + 2 * t + c);
+                float best = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < (HI ? 2 : 1); r++) {
-                const int ef = e + f[r], e1 = max(-126, min(127, ef));
-                const float s = (float)acc[2 * r + c] * exp2_int(e1) * exp2_int(ef - e1);
-                if (g + 8 * r < p.group) best = fmaxf(best, s);
+                for (int r = 0; r < NR; r++) {
+                    const int ef = e + f[r], e1 = max(-126, min(127, ef));
+                    const float x = (float)acc[2 * r + c] * exp2_int(e1) * exp2_int(ef - e1);
+                    if (g + 8 * r < p.group) best = fmaxf(best, x);
+                }
+                best = fmaxf(best, __shfl_xor_sync(FULL, best, 4));
+                best = fmaxf(best, __shfl_xor_sync(FULL, best, 8));
+                best = fmaxf(best, __shfl_xor_sync(FULL, best, 16));
+                // to the lane whose page it is (every lane of a column holds it)
+                const float mine = __shfl_sync(FULL, best, (lane >> 1) & 3);
+                if (lane >> 3 == in_window / 8 + k && (lane & 1) == c) key = ordered(mine);
             }
-            best = fmaxf(best, __shfl_xor_sync(FULL, best, 4));
-            best = fmaxf(best, __shfl_xor_sync(FULL, best, 8));
-            best = fmaxf(best, __shfl_xor_sync(FULL, best, 16));
-            const int pg = __shfl_sync(FULL, page, 4 * (2 * t + c)), idx = p0 + 2 * t + c;
-            if (g == 0 && idx < last)
-                keys[idx] = pg < 0 ? kKeyHole : (idx < p.first_pages || idx >= n - p.last_pages) ? kKeyForced : ordered(best);
+        }
+        __syncwarp();                                                       // the stage is free for the next request
+        if (in_window + SP == 32 || s == n_stages - 1) {
+            const int idx = begin + (s * SP & ~31) + lane;
+            if (idx < last)
+                keys[idx] = page32 < 0 ? kKeyHole : (idx < p.first_pages || idx >= n - p.last_pages) ? kKeyForced : key;
+            page32 = next32;
+            e32 = next_e;
+            next32 = checked(page_ids(begin + (s * SP & ~31) + 64));
+            next_e = exponent_of(next32);
         }
     }
 }
 
 // One CTA per (KV head, sequence): the top_pages largest keys (ties: lowest page), pages ascending, -1 behind them.
-// The k-th largest key is found bit by bit from the top: how many keys reach the candidate decides the bit.
-constexpr int kSelectThreads = 512;
+// The k-th largest key is found by 8-bit digits from the first bit in which the keys differ (scores of one query share
+// their exponent: counting digits from the top would put them all into one bin), each pass over the keys that share the
+// digits found so far; as soon as a bin's keys are all needed or none is, the rest of the digits does not matter.
+// Then every thread takes a run of pages and one scan gives each its places.
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
 __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const SelectParams p, int smem_keys) {
     extern __shared__ uint32_t s_keys[];
-    __shared__ int2 s_warp[kSelectThreads / 32];
+    __shared__ int s_bins[256];
+    __shared__ int s_int[2][kSelectWarps];
+    __shared__ uint32_t s_min[kSelectWarps], s_max[kSelectWarps];
+    __shared__ int s_pick[2];                                               // digit of the cut, keys still needed in its bin
     pdl_wait();
     pdl_launch_dependents();
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
@@ -317,72 +378,136 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const Selec
     const int n = len <= 0 || row < 0 || row >= p.max_rows ? 0 : min((len - 1) / p.page_size + 1, p.table_stride);
     const uint32_t* keys = p.keys + pair * p.key_stride;
     int32_t* sel = p.sel + pair * p.top_pages;
-    int mine = 0;
+    // ---- keys into shared memory; how many are resident, how many forced, and the others' range ----
+    int resident = 0, forced = 0;
+    uint32_t lo = 0xffffffffu, hi = 0;
+#pragma unroll 4
     for (int i = tid; i < n; i += kSelectThreads) {
-        const uint32_t k = keys[i];
+        const uint32_t k = __ldcg(keys + i);
         if (i < smem_keys) s_keys[i] = k;
-        mine += k != kKeyHole;
+        resident += k != kKeyHole;
+        forced += k == kKeyForced;
+        if (k != kKeyHole && k != kKeyForced) {
+            lo = min(lo, k);
+            hi = max(hi, k);
+        }
     }
-    auto key_at = [&](int i) { return i < smem_keys ? s_keys[i] : keys[i]; };
-    auto block_sum = [&](int v) -> int {
-        v = __reduce_add_sync(FULL, v);
-        __syncthreads();
-        if (lane == 0) s_warp[w].x = v;
-        __syncthreads();
-        int s = 0;
+    resident = __reduce_add_sync(FULL, resident);
+    forced = __reduce_add_sync(FULL, forced);
+    lo = __reduce_min_sync(FULL, lo);
+    hi = __reduce_max_sync(FULL, hi);
+    if (lane == 0) {
+        s_int[0][w] = resident;
+        s_int[1][w] = forced;
+        s_min[w] = lo;
+        s_max[w] = hi;
+    }
+    for (int i = tid; i < 256; i += kSelectThreads) s_bins[i] = 0;
+    __syncthreads();
+    resident = forced = 0;
 #pragma unroll
-        for (int i = 0; i < kSelectThreads / 32; i++) s += s_warp[i].x;
-        return s;
-    };
-    const int resident = block_sum(mine);
+    for (int i = 0; i < kSelectWarps; i++) {
+        resident += s_int[0][i];
+        forced += s_int[1][i];
+        lo = min(lo, s_min[i]);
+        hi = max(hi, s_max[i]);
+    }
+    auto key_at = [&](int i) { return i < smem_keys ? s_keys[i] : __ldcg(keys + i); };
     const int k = min(p.top_pages, resident);
-    uint32_t cut = 1;                                                       // everything resident
-    int above = 0;                                                          // keys > cut
+    // Taken are keys > cut_hi, and of those in [cut_lo, cut_hi] the first `ties` by page (more than there are: all).
+    uint32_t cut_lo = 1, cut_hi = 0;                                        // everything resident
+    int ties = 0;
     if (resident > k) {
-        cut = 0;
-        int reach = resident;                                               // keys >= cut, cut's lower bits being 0
-        for (int bit = 31; bit >= 0 && reach > k; bit--) {
-            const uint32_t cand = cut | (1u << bit);
-            int c = 0;
-            for (int i = tid; i < n; i += kSelectThreads) c += key_at(i) >= cand;
-            c = block_sum(c);
-            if (c >= k) {
-                cut = cand;
-                reach = c;
-            }
-        }
-        int c = 0;
-        for (int i = tid; i < n; i += kSelectThreads) c += key_at(i) > cut;
-        above = block_sum(c);
-        if (reach == k) above = -1;                                         // exactly k keys reach the cut: no ties to break
-    }
-    const int ties = above < 0 || resident == k ? n : k - above;            // keys equal to the cut that are taken, lowest first
-    const bool all = above < 0 || resident == k;
-    int done = 0, tied = 0;
-    for (int base = 0; base < n; base += kSelectThreads) {
-        const int i = base + tid;
-        const uint32_t key = i < n ? key_at(i) : kKeyHole;
-        const bool eq = !all && key == cut && key != kKeyHole;
-        const bool gt = key != kKeyHole && (all ? key >= cut : key > cut);
-        const uint32_t beq = __ballot_sync(FULL, eq), bgt = __ballot_sync(FULL, gt);
-        __syncthreads();
-        if (lane == 0) s_warp[w] = make_int2(__popc(bgt), __popc(beq));
-        __syncthreads();
-        int gt_before = done, eq_before = tied;
+        int need = k - forced;                                              // of the keys in [lo, hi]
+        if (need <= 0 || lo > hi) {
+            cut_lo = cut_hi = kKeyForced;                                   // forced ones only, the first k
+            ties = k;
+        } else {
+            int shift = lo == hi ? 0 : 32 - __clz(lo ^ hi);                 // bits from here on down differ
+            uint32_t prefix = shift >= 32 ? 0u : hi >> shift << shift;      // shared by all candidates
+            cut_lo = prefix;
+            cut_hi = hi;
+            while (shift > 0) {
+                const int down = shift < 8 ? 0 : shift - 8, bits = shift - down;
+                for (int i = tid; i < n; i += kSelectThreads) {
+                    const uint32_t key = key_at(i);
+                    if (key >= cut_lo && key <= cut_hi) atomicAdd(&s_bins[(key >> down) & ((1u << bits) - 1)], 1);
+                }
+                __syncthreads();
+                if (w == 0) {                                               // lane's bins: 255 - 8 lane .. 248 - 8 lane, from the top
+                    int c[8], sum = 0;
 #pragma unroll
-        for (int v = 0; v < kSelectThreads / 32; v++) {
-            if (v < w) {
-                gt_before += s_warp[v].x;
-                eq_before += s_warp[v].y;
+                    for (int i = 0; i < 8; i++) {
+                        c[i] = s_bins[255 - 8 * lane - i];
+                        sum += c[i];
+                    }
+                    int above = sum;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int v = __shfl_up_sync(FULL, above, o);
+                        if (lane >= o) above += v;
+                    }
+                    above -= sum;                                           // keys in bins above the lane's
+                    if (above < need && above + sum >= need) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            if (above < need && above + c[i] >= need) {
+                                s_pick[0] = 255 - 8 * lane - i;
+                                s_pick[1] = need - above;
+                            }
+                            above += c[i];
+                        }
+                    }
+                }
+                __syncthreads();
+                const int digit = s_pick[0], in_bin = s_bins[digit];
+                need = s_pick[1];
+                __syncthreads();
+                for (int i = tid; i < 256; i += kSelectThreads) s_bins[i] = 0;
+                __syncthreads();
+                cut_lo |= (uint32_t)digit << down;
+                cut_hi = cut_lo | ((1u << down) - 1);
+                shift = down;
+                if (need == in_bin) break;                                  // the whole bin is taken
             }
-            done += s_warp[v].x;
-            tied += s_warp[v].y;
+            ties = need;
         }
-        const uint32_t below = (1u << lane) - 1;
-        gt_before += __popc(bgt & below);
-        eq_before += __popc(beq & below);
-        const int at = gt_before + min(eq_before, ties);
-        if ((gt || (eq && eq_before < ties)) && at < k) sel[at] = i;
+    }
+    // ---- places: a run of pages per thread ----
+    const int run = (n + kSelectThreads - 1) / kSelectThreads, i0 = min(n, tid * run), i1 = min(n, i0 + run);
+    const bool all = resident == k;
+    int gt = 0, eq = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t key = key_at(i);
+        gt += all ? key != kKeyHole : key > cut_hi;
+        eq += !all && key >= cut_lo && key <= cut_hi;
+    }
+    int gt_in = gt, eq_in = eq;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(FULL, gt_in, o), c = __shfl_up_sync(FULL, eq_in, o);
+        if (lane >= o) {
+            gt_in += a;
+            eq_in += c;
+        }
+    }
+    __syncthreads();
+    if (lane == 31) {
+        s_int[0][w] = gt_in;
+        s_int[1][w] = eq_in;
+    }
+    __syncthreads();
+    int gt_at = gt_in - gt, eq_at = eq_in - eq;
+    for (int i = 0; i < w; i++) {
+        gt_at += s_int[0][i];
+        eq_at += s_int[1][i];
+    }
+    for (int i = i0; i < i1; i++) {
+        const uint32_t key = key_at(i);
+        const bool is_gt = all ? key != kKeyHole : key > cut_hi, is_eq = !all && key >= cut_lo && key <= cut_hi;
+        if (is_gt || (is_eq && eq_at < ties)) sel[gt_at + min(eq_at, ties)] = i;
+        gt_at += is_gt;
+        eq_at += is_eq;
     }
     for (int i = k + tid; i < p.top_pages; i += kSelectThreads) sel[i] = -1;
 }
@@ -400,12 +525,25 @@ cudaError_t launch_bounds_d(const BoundsParams& p, int head_dim, dim3 grid, cuda
 template <typename T, int D>
 cudaError_t launch_score(const SelectParams& p, int num_sms, cudaStream_t s) {
     const int pages = min((p.max_kv_len - 1) / p.page_size + 1, p.table_stride);
-    // a CTA takes 8 pages a warp at a time; more per CTA (the query bytes are made once) while 8 CTAs an SM remain
-    int per_cta = 8 * kScoreWarps;
-    while (per_cta < 1024 && (int64_t)((pages + 2 * per_cta - 1) / (2 * per_cta)) * p.num_kv_heads * p.n_seq >= 8 * num_sms) per_cta *= 2;
-    const dim3 grid((pages + per_cta - 1) / per_cta, p.num_kv_heads, p.n_seq);
-    return p.group > 8 ? launch_pdl(page_score_kernel<T, D, true>, grid, dim3(kScoreWarps * 32), 0, s, p, per_cta)
-                       : launch_pdl(page_score_kernel<T, D, false>, grid, dim3(kScoreWarps * 32), 0, s, p, per_cta);
+    int heads = kScoreWarps;
+    while (p.num_kv_heads % heads) heads >>= 1;
+    // 32 pages a warp; more (the query bytes are made once a warp) while CTAs for three turns of three an SM remain
+    int per_cta = 32 * (kScoreWarps / heads);
+    const int64_t ctas = (int64_t)(p.num_kv_heads / heads) * p.n_seq;
+    while (per_cta < 4096 && (pages + 2 * per_cta - 1) / (2 * per_cta) * ctas >= 9 * num_sms) per_cta *= 2;
+    const dim3 grid((pages + per_cta - 1) / per_cta, p.num_kv_heads / heads, p.n_seq);
+    constexpr size_t smem = (size_t)kScoreWarps * kScoreStages * kScoreStageBytes;
+    auto kernel = p.group > 8 ? page_score_kernel<T, D, true> : page_score_kernel<T, D, false>;
+    static std::atomic<bool> configured[64][2];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64 || !configured[dev][p.group > 8].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) configured[dev][p.group > 8].store(true, std::memory_order_release);
+    }
+    return launch_pdl(kernel, grid, dim3(kScoreWarps * 32), smem, s, p, per_cta, heads);
 }
 
 }  // namespace
@@ -438,9 +576,9 @@ cudaError_t launch_select_pages(const SelectParams& p, int head_dim, int dtype, 
         }
         if (e != cudaSuccess) return e;
     }
-    // keys beyond 12 288 (48 KB) of a sequence are read from global memory (L2) in every round
+    // keys beyond 11 776 (46 KB) of a sequence are read from global memory (L2) in every round
     const int pages = p.max_kv_len > 0 ? min((p.max_kv_len - 1) / p.page_size + 1, p.table_stride) : 0;
-    const int smem_keys = pages < 12288 - 256 ? pages : 12288 - 256;
+    const int smem_keys = pages < 11776 ? pages : 11776;
     return launch_pdl(page_select_kernel, dim3(p.num_kv_heads, p.n_seq), dim3(kSelectThreads), (size_t)smem_keys * 4, stream, p, smem_keys);
 }
 

@@ -57,6 +57,21 @@ struct RopeParams {
 
 __device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t magic) { return magic ? __umulhi(n, magic) : n; }
 
+// Cosines and sines of a CTA's tokens, one per thread.
+__device__ __forceinline__ void fill_trig(const RopeParams& p, float* s_trig, int tok0, int n_tok, int pad) {
+    for (int i = threadIdx.x; i < n_tok * pad; i += kRopeThreads) {
+        const int t = i / pad, j = i - t * pad;
+        if (j < p.half) {
+            const uint64_t phase = (uint64_t)(int64_t)__ldg(p.pos + tok0 + t) * __ldg(p.turns + j);
+            const int hi = (int)(uint32_t)((phase + 0x80000000ull) >> 32);
+            float s, c;
+            sincospif((float)hi * 0x1p-31f, &s, &c);
+            s_trig[t * 2 * pad + j] = c * p.factor;
+            s_trig[t * 2 * pad + pad + j] = (p.inverse ? -s : s) * p.factor;
+        }
+    }
+}
+
 template <int VW> struct RopeVec;
 template <> struct RopeVec<8> { using type = uint4; };
 template <> struct RopeVec<4> { using type = uint2; };
@@ -76,17 +91,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
     const int half = p.half, pad = (half + 3) & ~3;
     const int tok0 = blockIdx.x * p.tokens_per_cta;
     const int n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
-    for (int i = threadIdx.x; i < n_tok * pad; i += kRopeThreads) {
-        const int t = i / pad, j = i - t * pad;
-        if (j < half) {
-            const uint64_t phase = (uint64_t)(int64_t)__ldg(p.pos + tok0 + t) * __ldg(p.turns + j);
-            const int hi = (int)(uint32_t)((phase + 0x80000000ull) >> 32);
-            float s, c;
-            sincospif((float)hi * 0x1p-31f, &s, &c);
-            s_trig[t * 2 * pad + j] = c * p.factor;
-            s_trig[t * 2 * pad + pad + j] = (p.inverse ? -s : s) * p.factor;
-        }
-    }
+    fill_trig(p, s_trig, tok0, n_tok, pad);
     __syncthreads();
     const uint32_t per_token = (uint32_t)p.heads * p.row_items, total = per_token * n_tok;
     for (uint32_t base = threadIdx.x; base < total; base += kRopeThreads * kRopeUnroll) {
@@ -150,6 +155,78 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
                 *reinterpret_cast<V*>(dst[u] + off_b[u]) = b[u];
             }
             *reinterpret_cast<V*>(dst[u]) = a[u];
+        }
+    }
+}
+
+// The usual heads (64, 128 or 256 dims, 16-byte vectors): a lane takes one vector of a row, its partners of the other half
+// come by shuffle (pairs: they are in the same vector), and four rows a lane are read before the first is worked on.
+// What the general kernel below loses on them is index arithmetic per vector: 32 768 tokens of 40 heads of 128 took 158 us there.
+template <typename T, bool PAIRS>
+__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+    extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][half_pad]
+    pdl_wait();
+    pdl_launch_dependents();
+    const int half = p.half, pad = (half + 3) & ~3;
+    const int tok0 = blockIdx.x * p.tokens_per_cta, n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
+    fill_trig(p, s_trig, tok0, n_tok, pad);
+    __syncthreads();
+    const int lanes = 1 << lanes_log2, l = threadIdx.x & (lanes - 1), rows_at_once = kRopeThreads >> lanes_log2;
+    const int total = n_tok * p.heads, rot_lanes = p.rotary_dim >> 3, half_lanes = half >> 3;
+    const bool turns = l < rot_lanes;
+    const bool second = !PAIRS && l >= half_lanes;
+    const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
+    const int trig0 = turns ? (PAIRS ? 4 * l : 8 * (second ? l - half_lanes : l)) : 0;
+    for (int r0 = threadIdx.x >> lanes_log2; r0 < total + (int)(threadIdx.x >> lanes_log2); r0 += kRopeUnroll * rows_at_once) {   // the whole CTA together
+        Vec16 v[kRopeUnroll];
+        T* dst[kRopeUnroll];
+        int tok[kRopeUnroll];
+#pragma unroll
+        for (int u = 0; u < kRopeUnroll; u++) {
+            const int row = r0 + u * rows_at_once;
+            dst[u] = nullptr;
+            tok[u] = 0;
+            v[u] = Vec16{{0u, 0u, 0u, 0u}};
+            if (row >= total) continue;
+            const int t = div_magic(row, p.magic_heads), h = row - t * p.heads;
+            const bool is_k = h >= p.q_heads;
+            const RopeRowsDev& r = is_k ? p.k : p.q;
+            if (!turns && r.src == r.dst) continue;             // in place, and these dims stay
+            const int64_t head = is_k ? h - p.q_heads : h;
+            v[u] = ldg16(reinterpret_cast<const T*>(r.src) + (int64_t)(tok0 + t) * r.src_token + head * r.src_head + 8 * l);
+            dst[u] = reinterpret_cast<T*>(r.dst) + (int64_t)(tok0 + t) * r.dst_token + head * r.dst_head + 8 * l;
+            tok[u] = t;
+        }
+#pragma unroll
+        for (int u = 0; u < kRopeUnroll; u++) {
+            const float4* cs = reinterpret_cast<const float4*>(s_trig + tok[u] * 2 * pad + trig0);   // 16-byte aligned: half % 4 == 0
+            float c[8], s[8];
+#pragma unroll
+            for (int i = 0; i < (PAIRS ? 1 : 2); i++) {
+                *reinterpret_cast<float4*>(c + 4 * i) = cs[i];
+                *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + i];
+            }
+            Vec16 y;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 x = Elem<T>::unpack2(v[u].w[i]);
+                float y0, y1, dead;
+                (void)dead;
+                if (PAIRS) {
+                    rope_pair(x.x, x.y, c[i], s[i], y0, y1);
+                } else {
+                    const float2 o = Elem<T>::unpack2(__shfl_sync(0xffffffffu, v[u].w[i], partner));
+                    if (second) {
+                        rope_pair(o.x, x.x, c[2 * i], s[2 * i], dead, y0);
+                        rope_pair(o.y, x.y, c[2 * i + 1], s[2 * i + 1], dead, y1);
+                    } else {
+                        rope_pair(x.x, o.x, c[2 * i], s[2 * i], y0, dead);
+                        rope_pair(x.y, o.y, c[2 * i + 1], s[2 * i + 1], y1, dead);
+                    }
+                }
+                y.w[i] = turns ? Elem<T>::pack2(y0, y1) : v[u].w[i];
+            }
+            if (dst[u] != nullptr) stg16(dst[u], y);
         }
     }
 }
@@ -320,7 +397,7 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
     const int d = r->cfg.head_dim, rot = r->cfg.rotary_dim;
     int vw = 8;
     while (vw > 1 && (rot / 2) % vw != 0) vw >>= 1;
-    bool copies = false;
+    bool copies = false, wide_rows = true;                       // wide_rows: every row in 16-byte vectors
     for (const drkv_rope_rows* x : {q, k}) {
         if (!x || x->heads == 0) continue;
         if (x->heads < 0 || x->heads > 4096) return fail(DRKV_ERR_INVALID, "rope_apply: heads must be 0 to 4096");
@@ -350,6 +427,7 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
             copies = true;
         }
         vw = widest(*x, n_tokens, vw);
+        wide_rows &= widest(*x, n_tokens, 8) == 8;
     }
     const int qh = q ? q->heads : 0, kh = k ? k->heads : 0;
     if (n_tokens == 0 || qh + kh == 0) return DRKV_OK;
@@ -382,6 +460,18 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
     const size_t smem = (size_t)p.tokens_per_cta * 2 * ((p.half + 3) & ~3) * sizeof(float);
     DeviceGuard dev(r->cfg.device);
     if (!dev.ok()) return fail(DRKV_ERR_CUDA, "rope_apply: cudaSetDevice failed");
+    // the row kernel takes heads of 64, 128 and 256 dims (their lanes divide a warp) in 16-byte vectors
+    if (wide_rows && (d == 64 || d == 128 || d == 256) && rot % (r->cfg.layout == DRKV_ROPE_PAIRS ? 8 : 16) == 0) {
+        const int lg = d == 64 ? 3 : d == 128 ? 4 : 5;
+        const bool pairs = r->cfg.layout == DRKV_ROPE_PAIRS, f16 = r->cfg.dtype == DRKV_DTYPE_F16;
+        const cudaStream_t st = (cudaStream_t)stream;
+        const cudaError_t e = f16 ? (pairs ? launch_pdl(rope_rows_kernel<__half, true>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg)
+                                           : launch_pdl(rope_rows_kernel<__half, false>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg))
+                                  : (pairs ? launch_pdl(rope_rows_kernel<__nv_bfloat16, true>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg)
+                                           : launch_pdl(rope_rows_kernel<__nv_bfloat16, false>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg));
+        if (e != cudaSuccess) return fail(DRKV_ERR_CUDA, cudaGetErrorString(e));
+        return DRKV_OK;
+    }
     const cudaError_t ce = r->cfg.dtype == DRKV_DTYPE_F16 ? launch_rope<__half>(p, vw, grid, smem, (cudaStream_t)stream)
                                                           : launch_rope<__nv_bfloat16>(p, vw, grid, smem, (cudaStream_t)stream);
     if (ce != cudaSuccess) return fail(DRKV_ERR_CUDA, cudaGetErrorString(ce));
