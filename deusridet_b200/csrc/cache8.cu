@@ -104,10 +104,10 @@ struct TokenPlace {
     int slot, pos;
 };
 
-// A CTA takes some tokens, D / 8 lanes per row: a token's K heads, then its V heads, as in its page block.  BATCH rows a lane
-// are read before the first is worked on (a row at a time, one token per CTA: 30 000 tokens of 4 heads of 256 took 77 us).
-template <typename T, int D, int BATCH>
-__global__ void __launch_bounds__(kThreads8) append8_kernel(const Append8Params p, int n_all, int tokens_per_cta, uint32_t magic_rows) {
+// A CTA takes some tokens, D / 8 lanes per row: a token's K heads, then its V heads, as in its page block.  The next row is
+// on its way while one is worked on (30 001 tokens of 4 heads of 256: 41 us, 4.5 TB/s; one token a CTA and no read ahead: 77).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads8, 6) append8_kernel(const Append8Params p, int n_all, int tokens_per_cta, uint32_t magic_rows) {
     constexpr int LANES = D / 8, ROWS = kThreads8 / LANES;
     extern __shared__ float s_trig[];                                // [token][2][half]
     __shared__ TokenPlace s_place[kMaxTokens8];
@@ -117,20 +117,14 @@ __global__ void __launch_bounds__(kThreads8) append8_kernel(const Append8Params 
     const int P = p.layout.page_size, H = p.layout.num_kv_heads;
     const int l = threadIdx.x % LANES, total = n_tok * 2 * H;
     const int64_t exponents = 2 * p.layout.plane;
-    Vec16 in[BATCH];
-    auto read = [&](int r0) {
-#pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int r = r0 + u * ROWS;
-            in[u] = Vec16{{0u, 0u, 0u, 0u}};
-            if (r < total) {
-                const int t = div_magic(r, magic_rows), kh = r - t * 2 * H;
-                const T* src = reinterpret_cast<const T*>(kh < H ? p.k_src : p.v_src) + ((int64_t)(tok0 + t) * H + (kh < H ? kh : kh - H)) * D;
-                in[u] = ldg16(src + 8 * l);
-            }
-        }
+    auto read = [&](int r) -> Vec16 {
+        if (r >= total) return Vec16{{0u, 0u, 0u, 0u}};
+        const int t = div_magic(r, magic_rows), kh = r - t * 2 * H;
+        const T* src = reinterpret_cast<const T*>(kh < H ? p.k_src : p.v_src) + ((int64_t)(tok0 + t) * H + (kh < H ? kh : kh - H)) * D;
+        return ldg16(src + 8 * l);
     };
-    read(threadIdx.x / LANES);                                       // on their way while the places are worked out
+    const int r_own = threadIdx.x / LANES;
+    Vec16 a = read(r_own), b;                                        // on its way while the places are worked out
     if (threadIdx.x < n_tok) {
         const int tok = tok0 + threadIdx.x;
         int row = p.row, pos = p.pos_start + tok;
@@ -154,33 +148,35 @@ __global__ void __launch_bounds__(kThreads8) append8_kernel(const Append8Params 
         }
         __syncthreads();
     }
-    for (int r0 = threadIdx.x / LANES; r0 < total + threadIdx.x / LANES; r0 += BATCH * ROWS) {   // the whole CTA together
+    auto write = [&](const Vec16& in, int r) {
+        const int t = div_magic(min(r, total - 1), magic_rows), kh = min(r, total - 1) - t * 2 * H;
+        float x[8];
+        unpack8<T>(in, x);
+        if (half > 0) {
+            const int hl = half / 8;                                 // lanes of one rotated half (rotary_dim % 16 == 0)
+            const bool first = l < hl, second = l >= hl && l < 2 * hl;
+            // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
+            const int base = (threadIdx.x & 31) - l, other = base + (first ? l + hl : second ? l - hl : l);
+            const float* c = s_trig + 2 * t * half + 8 * (first ? l : second ? l - hl : 0);
 #pragma unroll
-        for (int u = 0; u < BATCH; u++) {
-            const int r = r0 + u * ROWS;
-            const int t = div_magic(min(r, total - 1), magic_rows), kh = min(r, total - 1) - t * 2 * H;
-            float x[8];
-            unpack8<T>(in[u], x);
-            if (half > 0) {
-                const int hl = half / 8;                             // lanes of one rotated half (rotary_dim % 16 == 0)
-                const bool first = l < hl, second = l >= hl && l < 2 * hl;
-                // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
-                const int base = (threadIdx.x & 31) - l, other = base + (first ? l + hl : second ? l - hl : l);
-                const float* c = s_trig + 2 * t * half + 8 * (first ? l : second ? l - hl : 0);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float o = __shfl_sync(0xffffffffu, x[i], other);
-                    if (kh < H && (first || second)) {
-                        float y0, y1;
-                        rope_pair(first ? x[i] : o, first ? o : x[i], c[i], c[half + i], y0, y1);
-                        x[i] = first ? y0 : y1;
-                    }
+            for (int i = 0; i < 8; i++) {
+                const float o = __shfl_sync(0xffffffffu, x[i], other);
+                if (kh < H && (first || second)) {
+                    float y0, y1;
+                    rope_pair(first ? x[i] : o, first ? o : x[i], c[i], c[half + i], y0, y1);
+                    x[i] = first ? y0 : y1;
                 }
             }
-            const TokenPlace at = s_place[t];
-            quantise_row<LANES>(x, p.pool + at.block, exponents, kh * P + at.slot, l, r < total && at.block >= 0);
         }
-        read(r0 + BATCH * ROWS);
+        const TokenPlace at = s_place[t];
+        quantise_row<LANES>(x, p.pool + at.block, exponents, kh * P + at.slot, l, r < total && at.block >= 0);
+    };
+    for (int r0 = 0; r0 < total; r0 += 2 * ROWS) {                   // the whole CTA together: rows r0 + r_own, then the next
+        b = read(r0 + ROWS + r_own);
+        write(a, r0 + r_own);
+        if (r0 + ROWS >= total) break;
+        a = read(r0 + 2 * ROWS + r_own);
+        write(b, r0 + ROWS + r_own);
     }
 }
 
@@ -313,17 +309,14 @@ cudaError_t by_shape(const P& p, int dtype, int head_dim, int n, cudaStream_t st
 template <typename T, int D>
 struct AppendLaunch {
     static cudaError_t run(const Append8Params& p, int n, cudaStream_t s) {
-        // one row a lane and one token a CTA for decode batches; four rows a lane, and the tokens for them, once such CTAs
-        // fill the SMs twice over (4 of 256 threads each)
+        // a token a CTA for decode batches; more, a dozen rows a lane and at most 32 tokens, while such CTAs fill the SMs twice
+        // over (6 of 256 threads each)
         constexpr int ROWS = kThreads8 / (D / 8);
         const int H = p.layout.num_kv_heads;
         int per = 1;
-        while (per < kMaxTokens8 && per * 2 * H < 4 * ROWS) per *= 2;
-        const uint32_t magic = magic_of(2 * H);
-        if (n < per * 4 * 2 * 148)
-            return launch_pdl(append8_kernel<T, D, 1>, dim3(n), dim3(kThreads8), p.rotary_dim * sizeof(float), s, p, n, 1, magic);
-        return launch_pdl(append8_kernel<T, D, 4>, dim3((n + per - 1) / per), dim3(kThreads8), (size_t)per * p.rotary_dim * sizeof(float),
-                          s, p, n, per, magic);
+        while (per < kMaxTokens8 && per * 2 * H < 12 * ROWS && n >= 2 * per * 2 * 6 * 148) per *= 2;
+        return launch_pdl(append8_kernel<T, D>, dim3((n + per - 1) / per), dim3(kThreads8), (size_t)per * p.rotary_dim * sizeof(float),
+                          s, p, n, per, magic_of(2 * H));
     }
 };
 template <typename T, int D>

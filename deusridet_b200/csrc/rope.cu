@@ -33,7 +33,7 @@ namespace drkv {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeUnroll = 4;       // items a thread has in flight
+constexpr int kRopeUnroll = 4;       // items a thread of the general kernel has in flight
 
 struct RopeRowsDev {
     const void* src;
@@ -160,74 +160,76 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 }
 
 // The usual heads (64, 128 or 256 dims, 16-byte vectors): a lane takes one vector of a row, its partners of the other half
-// come by shuffle (pairs: they are in the same vector), and four rows a lane are read before the first is worked on.
-// What the general kernel below loses on them is index arithmetic per vector: 32 768 tokens of 40 heads of 128 took 158 us there.
+// come by shuffle (pairs: they are in the same vector), and the next row is on its way while one is worked on.  32 registers, so
+// that 2 048 threads an SM keep loads in flight: 32 768 tokens of 40 heads of 128 122 us (5.5 TB/s); four rows a lane at 80
+// registers: 138.
+// (The general kernel above loses on them by index arithmetic per vector: 158 us.)
 template <typename T, bool PAIRS>
-__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+__global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopeParams p, int lanes_log2) {
     extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][half_pad]
     pdl_wait();
     pdl_launch_dependents();
     const int half = p.half, pad = (half + 3) & ~3;
     const int tok0 = blockIdx.x * p.tokens_per_cta, n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
-    fill_trig(p, s_trig, tok0, n_tok, pad);
-    __syncthreads();
     const int lanes = 1 << lanes_log2, l = threadIdx.x & (lanes - 1), rows_at_once = kRopeThreads >> lanes_log2;
     const int total = n_tok * p.heads, rot_lanes = p.rotary_dim >> 3, half_lanes = half >> 3;
     const bool turns = l < rot_lanes;
     const bool second = !PAIRS && l >= half_lanes;
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
     const int trig0 = turns ? (PAIRS ? 4 * l : 8 * (second ? l - half_lanes : l)) : 0;
-    for (int r0 = threadIdx.x >> lanes_log2; r0 < total + (int)(threadIdx.x >> lanes_log2); r0 += kRopeUnroll * rows_at_once) {   // the whole CTA together
-        Vec16 v[kRopeUnroll];
-        T* dst[kRopeUnroll];
-        int tok[kRopeUnroll];
+    struct Row {
+        Vec16 v;
+        T* dst;                                                 // null: nothing to write
+        int tok;
+    };
+    auto read = [&](int row) -> Row {
+        Row x{Vec16{{0u, 0u, 0u, 0u}}, nullptr, 0};
+        if (row >= total) return x;
+        const int t = div_magic(row, p.magic_heads), h = row - t * p.heads;
+        const bool is_k = h >= p.q_heads;
+        const RopeRowsDev& r = is_k ? p.k : p.q;
+        if (!turns && r.src == r.dst) return x;                 // in place, and these dims stay
+        const int64_t head = is_k ? h - p.q_heads : h;
+        x.v = ldg16(reinterpret_cast<const T*>(r.src) + (int64_t)(tok0 + t) * r.src_token + head * r.src_head + 8 * l);
+        x.dst = reinterpret_cast<T*>(r.dst) + (int64_t)(tok0 + t) * r.dst_token + head * r.dst_head + 8 * l;
+        x.tok = t;
+        return x;
+    };
+    auto write = [&](const Row& x) {
+        const float4* cs = reinterpret_cast<const float4*>(s_trig + x.tok * 2 * pad + trig0);   // 16-byte aligned: half % 4 == 0
+        float c[8], s[8];
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; u++) {
-            const int row = r0 + u * rows_at_once;
-            dst[u] = nullptr;
-            tok[u] = 0;
-            v[u] = Vec16{{0u, 0u, 0u, 0u}};
-            if (row >= total) continue;
-            const int t = div_magic(row, p.magic_heads), h = row - t * p.heads;
-            const bool is_k = h >= p.q_heads;
-            const RopeRowsDev& r = is_k ? p.k : p.q;
-            if (!turns && r.src == r.dst) continue;             // in place, and these dims stay
-            const int64_t head = is_k ? h - p.q_heads : h;
-            v[u] = ldg16(reinterpret_cast<const T*>(r.src) + (int64_t)(tok0 + t) * r.src_token + head * r.src_head + 8 * l);
-            dst[u] = reinterpret_cast<T*>(r.dst) + (int64_t)(tok0 + t) * r.dst_token + head * r.dst_head + 8 * l;
-            tok[u] = t;
+        for (int i = 0; i < (PAIRS ? 1 : 2); i++) {
+            *reinterpret_cast<float4*>(c + 4 * i) = cs[i];
+            *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + i];
         }
+        Vec16 y;
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; u++) {
-            const float4* cs = reinterpret_cast<const float4*>(s_trig + tok[u] * 2 * pad + trig0);   // 16-byte aligned: half % 4 == 0
-            float c[8], s[8];
-#pragma unroll
-            for (int i = 0; i < (PAIRS ? 1 : 2); i++) {
-                *reinterpret_cast<float4*>(c + 4 * i) = cs[i];
-                *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + i];
+        for (int i = 0; i < 4; i++) {
+            const float2 own = Elem<T>::unpack2(x.v.w[i]);
+            float y0, y1;
+            if (PAIRS) {
+                rope_pair(own.x, own.y, c[i], s[i], y0, y1);
+            } else {
+                const float2 o = Elem<T>::unpack2(__shfl_sync(0xffffffffu, x.v.w[i], partner));
+                // first half: x0 c - x1 s; second: x1 c + x0 s
+                y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, second ? s[2 * i] : -s[2 * i]));
+                y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, second ? s[2 * i + 1] : -s[2 * i + 1]));
             }
-            Vec16 y;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float2 x = Elem<T>::unpack2(v[u].w[i]);
-                float y0, y1, dead;
-                (void)dead;
-                if (PAIRS) {
-                    rope_pair(x.x, x.y, c[i], s[i], y0, y1);
-                } else {
-                    const float2 o = Elem<T>::unpack2(__shfl_sync(0xffffffffu, v[u].w[i], partner));
-                    if (second) {
-                        rope_pair(o.x, x.x, c[2 * i], s[2 * i], dead, y0);
-                        rope_pair(o.y, x.y, c[2 * i + 1], s[2 * i + 1], dead, y1);
-                    } else {
-                        rope_pair(x.x, o.x, c[2 * i], s[2 * i], y0, dead);
-                        rope_pair(x.y, o.y, c[2 * i + 1], s[2 * i + 1], y1, dead);
-                    }
-                }
-                y.w[i] = turns ? Elem<T>::pack2(y0, y1) : v[u].w[i];
-            }
-            if (dst[u] != nullptr) stg16(dst[u], y);
+            y.w[i] = turns ? Elem<T>::pack2(y0, y1) : x.v.w[i];
         }
+        if (x.dst != nullptr) stg16(x.dst, y);
+    };
+    const int r_own = threadIdx.x >> lanes_log2;
+    Row a = read(r_own), b;                                     // on its way while the cosines are evaluated
+    fill_trig(p, s_trig, tok0, n_tok, pad);
+    __syncthreads();
+    for (int r0 = 0; r0 < total; r0 += 2 * rows_at_once) {      // the whole CTA together: rows r0 + r_own, then the next
+        b = read(r0 + rows_at_once + r_own);
+        write(a);
+        if (r0 + rows_at_once >= total) break;
+        a = read(r0 + 2 * rows_at_once + r_own);
+        write(b);
     }
 }
 

@@ -9,7 +9,7 @@ import numpy as np
 
 from . import capi
 from .capi import RopeConfig, RopeRows, check
-from .engine import _ptr, _stream
+from .engine import _stream
 
 LAYOUTS = {"halves": 0, "pairs": 1}
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
@@ -55,20 +55,14 @@ class Rope:
         return out
 
     def _rows(self, src, dst, n_tokens, name) -> RopeRows:
-        import torch
-        want = torch.float16 if self.dtype == capi.F16 else torch.bfloat16
-        for what, t in ((name, src), (f"out_{name}", dst)):
-            if t.dim() != 3 or t.shape[0] != n_tokens or t.shape[2] != self.head_dim:
-                raise ValueError(f"{what} must have shape [{n_tokens}, heads, {self.head_dim}], not {tuple(t.shape)}")
-            if t.dtype != want:
-                raise ValueError(f"{what} must be {want}, not {t.dtype}")
-            if t.device.type != "cuda" or t.device.index != self.device:
-                raise ValueError(f"{what} must be on cuda:{self.device}, not {t.device}")
-            if t.stride(2) != 1:
-                raise ValueError(f"the last dimension of {what} must be contiguous")
-        if dst.shape != src.shape:
-            raise ValueError(f"out_{name} must have the shape of {name}")
-        return RopeRows(_ptr(src), _ptr(dst), src.shape[1], src.stride(0), src.stride(1), dst.stride(0), dst.stride(1))
+        shape, strides, to_shape, to_strides = src.shape, src.stride(), dst.shape, dst.stride()
+        if (len(shape) != 3 or shape[0] != n_tokens or shape[2] != self.head_dim or to_shape != shape or
+                src.dtype is not self._torch_dtype or dst.dtype is not self._torch_dtype or strides[2] != 1 or to_strides[2] != 1 or
+                src.get_device() != self.device or dst.get_device() != self.device):
+            raise ValueError(f"{name} and out_{name} must be tensors [{n_tokens}, heads, {self.head_dim}] of {self._torch_dtype} on "
+                             f"cuda:{self.device} with a contiguous last dimension, not {tuple(shape)} {src.dtype} {src.device} and "
+                             f"{tuple(to_shape)} {dst.dtype} {dst.device}")
+        return RopeRows(src.data_ptr(), dst.data_ptr(), shape[1], strides[0], strides[1], to_strides[0], to_strides[1])
 
     def apply(self, pos, q=None, k=None, *, out_q=None, out_k=None, inverse: bool = False, stream=None):
         """Rotates q and k, tensors [n_tokens, heads, head_dim] of any token and head strides, by the int32 positions
@@ -77,21 +71,20 @@ class Rope:
         import torch
         if q is None and k is None:
             raise ValueError("nothing to rotate: give q, k or both")
-        if pos.dtype != torch.int32 or pos.dim() != 1 or not pos.is_contiguous() or pos.device.index != self.device:
+        if (q is None and out_q is not None) or (k is None and out_k is not None):
+            raise ValueError("an output without its input")
+        if pos.dtype is not torch.int32 or pos.dim() != 1 or not pos.is_contiguous() or pos.get_device() != self.device:
             raise ValueError(f"pos must be a contiguous int32 vector on cuda:{self.device}")
-        rows = []
-        outs = []
-        for name, src, dst in (("q", q, out_q), ("k", k, out_k)):
-            if src is None:
-                if dst is not None:
-                    raise ValueError(f"out_{name} without {name}")
-                rows.append(None)
-                outs.append(None)
-                continue
-            if dst is None:
-                dst = torch.empty(src.shape, dtype=src.dtype, device=src.device)
-            rows.append(self._rows(src, dst, pos.shape[0], name))
-            outs.append(dst)
-        ref = [None if r is None else C.byref(r) for r in rows]
-        check(self.lib.drkv_rope_apply(self.h, pos.shape[0], _ptr(pos), ref[0], ref[1], 1 if inverse else 0, _stream(stream)))
-        return outs[0], outs[1]
+        self._torch_dtype = torch.float16 if self.dtype == capi.F16 else torch.bfloat16
+        n = pos.shape[0]
+        q_rows = k_rows = None
+        if q is not None:
+            if out_q is None:
+                out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_rows = C.byref(self._rows(q, out_q, n, "q"))
+        if k is not None:
+            if out_k is None:
+                out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            k_rows = C.byref(self._rows(k, out_k, n, "k"))
+        check(self.lib.drkv_rope_apply(self.h, n, pos.data_ptr(), q_rows, k_rows, 1 if inverse else 0, _stream(stream)))
+        return out_q, out_k
