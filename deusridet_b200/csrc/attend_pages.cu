@@ -41,7 +41,7 @@ constexpr float kNoKey = -1.0e30f;    // running maximum before any key
 template <bool POOL8, int D, int NQ> struct Ring;
 template <int NQ> struct Ring<true, 64, NQ>   { static constexpr int kWarps = 16, kStages = 4; };   // 132 KB
 template <> struct Ring<true, 128, 1>         { static constexpr int kWarps = 16, kStages = 3; };   // 198 KB
-template <> struct Ring<true, 128, 2>         { static constexpr int kWarps = 8, kStages = 5; };    // 165 KB
+template <> struct Ring<true, 128, 2>         { static constexpr int kWarps = 12, kStages = 4; };   // 198 KB
 template <int NQ> struct Ring<true, 256, NQ>  { static constexpr int kWarps = 8, kStages = 3; };    // 197 KB
 template <int NQ> struct Ring<false, 64, NQ>  { static constexpr int kWarps = 16, kStages = 3; };   // 192 KB
 template <int NQ> struct Ring<false, 128, NQ> { static constexpr int kWarps = 8, kStages = 3; };    // 192 KB
@@ -682,11 +682,16 @@ cudaError_t launch_one(const AttendPagesParams& p, int num_sms, cudaStream_t str
     if (e != cudaSuccess) return e;
     const int n_warps = num_sms * R::kWarps;
     const int64_t pairs = (int64_t)p.n_seq * p.num_kv_heads, rows = pairs * p.group;
-    // about n_warps / pairs pieces a row; few rows are spread over CTAs of 32 dims (32 rows of 296 pieces: 8 us against 9,
-    // 512 rows of 37 pieces: 19 us against 7 by whole rows)
-    if (rows * (D / 32) <= 2 * num_sms)
+    // About n_warps / pairs pieces a row, eight of which a set of lanes takes at a time: the more pieces, the fewer dims a CTA
+    // takes and the more sets it has (60 rows of 118 pieces of 256 dims: 20 us a pass with four sets, 15 with thirty-two).
+    const int64_t pieces = n_warps / pairs + 2;
+    if (pieces > 8) {
+        constexpr int MID = D > 64 ? 64 : D;
+        if (pieces <= 8 * (1024 / D)) return launch_pdl(merge_pieces_kernel<T, D, D>, dim3((unsigned)rows), dim3(256), 0, stream, p, n_warps);
+        if (pieces <= 8 * (1024 / MID))
+            return launch_pdl(merge_pieces_kernel<T, D, MID>, dim3((unsigned)rows, D / MID), dim3(256), 0, stream, p, n_warps);
         return launch_pdl(merge_pieces_kernel<T, D, 32>, dim3((unsigned)rows, D / 32), dim3(256), 0, stream, p, n_warps);
-    if (pairs * 8 < n_warps) return launch_pdl(merge_pieces_kernel<T, D, D>, dim3((unsigned)rows), dim3(256), 0, stream, p, n_warps);
+    }
     constexpr int per_cta = 128 / (D / 4);
     return launch_pdl(merge_pieces_kernel<T, D, 0>, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(128), 0, stream, p, n_warps);
 }

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
     const int half = p.half, pad = (half + 3) & ~3;
     const int tok0 = blockIdx.x * p.tokens_per_cta, n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
     const int lanes = 1 << lanes_log2, l = threadIdx.x & (lanes - 1), rows_at_once = kRopeThreads >> lanes_log2;
-    const int total = n_tok * p.heads, rot_lanes = p.rotary_dim >> 3, half_lanes = half >> 3;
+    const int total = n_tok * p.heads, rot_lanes = (p.rotary_dim + 7) >> 3, half_lanes = half >> 3;
     const bool turns = l < rot_lanes;
     const bool second = !PAIRS && l >= half_lanes;
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
         return x;
     };
     auto write = [&](const Row& x) {
-        const float4* cs = reinterpret_cast<const float4*>(s_trig + x.tok * 2 * pad + trig0);   // 16-byte aligned: half % 4 == 0
+        const float4* cs = reinterpret_cast<const float4*>(s_trig + x.tok * 2 * pad + trig0);   // 16-byte aligned: pad % 4 == 0
         float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < (PAIRS ? 1 : 2); i++) {
@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
                 y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, second ? s[2 * i] : -s[2 * i]));
                 y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, second ? s[2 * i + 1] : -s[2 * i + 1]));
             }
-            y.w[i] = turns ? Elem<T>::pack2(y0, y1) : x.v.w[i];
+            // (pairs: the last vector that turns may hold pairs that do not)
+            y.w[i] = turns && (!PAIRS || 4 * l + i < half) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
         }
         if (x.dst != nullptr) stg16(x.dst, y);
     };
@@ -463,7 +464,7 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
     DeviceGuard dev(r->cfg.device);
     if (!dev.ok()) return fail(DRKV_ERR_CUDA, "rope_apply: cudaSetDevice failed");
     // the row kernel takes heads of 64, 128 and 256 dims (their lanes divide a warp) in 16-byte vectors
-    if (wide_rows && (d == 64 || d == 128 || d == 256) && rot % (r->cfg.layout == DRKV_ROPE_PAIRS ? 8 : 16) == 0) {
+    if (wide_rows && (d == 64 || d == 128 || d == 256) && (r->cfg.layout == DRKV_ROPE_PAIRS || rot % 16 == 0)) {
         const int lg = d == 64 ? 3 : d == 128 ? 4 : 5;
         const bool pairs = r->cfg.layout == DRKV_ROPE_PAIRS, f16 = r->cfg.dtype == DRKV_DTYPE_F16;
         const cudaStream_t st = (cudaStream_t)stream;
