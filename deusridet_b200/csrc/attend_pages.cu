@@ -35,7 +35,7 @@ namespace drkv {
 
 namespace {
 
-constexpr float kNoKey = -1.0e30f;    // running maximum before any key
+constexpr float kNoKey = -3.402823466e38f;   // running maximum before any key: no finite score is below it
 
 // Warps per CTA (one CTA per SM) and groups in a warp's ring.
 template <bool POOL8, int D, int NQ> struct Ring;
@@ -418,8 +418,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
 #pragma unroll
             for (int k = 0; k < 4; k++) s[0][k] += s2[k];
         }
-        // s * f is the score in the log2 domain.  A K row whose byte is 0 (everything below 2^-118) counts as zeros.
-        float f0[NQ][2], f1[NQ][2];
+        // s becomes the score in the log2 domain.  A K row whose byte is 0 (everything below 2^-118) counts as zeros.
         uint32_t ev0 = 0, ev1 = 0;
         float ks0 = 1.f, ks1 = 1.f;
         if (POOL8) {
@@ -439,9 +438,12 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                f0[nq][c] = POOL8 ? ks0 * qs[nq][c] : qs[nq][c];
-                f1[nq][c] = POOL8 ? ks1 * qs[nq][c] : qs[nq][c];
-                grow |= fmaxf(fmaf(s[nq][c], f0[nq][c], -m[nq][c]), fmaf(s[nq][2 + c], f1[nq][c], -m[nq][c])) > kSlack;
+                const float f0 = POOL8 ? ks0 * qs[nq][c] : qs[nq][c], f1 = POOL8 ? ks1 * qs[nq][c] : qs[nq][c];
+                // the product is rounded before the maximum is taken off, as the maximum was: of scores beyond 2^27 a fused
+                // product's lower half alone could exceed the slack
+                s[nq][c] = __fmul_rn(s[nq][c], f0);
+                s[nq][2 + c] = __fmul_rn(s[nq][2 + c], f1);
+                grow |= __fadd_rn(fmaxf(s[nq][c], s[nq][2 + c]), -m[nq][c]) > kSlack;
             }
         if (__any_sync(FULL, grow)) {
             const int new_e = POOL8 ? max(big_e, __reduce_max_sync(FULL, (int)max(ev0, ev1))) : 0;
@@ -453,7 +455,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    float x = fmaxf(g < valid ? s[nq][c] * f0[nq][c] : -INFINITY, g + 8 < valid ? s[nq][2 + c] * f1[nq][c] : -INFINITY);
+                    float x = fmaxf(g < valid ? s[nq][c] : -INFINITY, g + 8 < valid ? s[nq][2 + c] : -INFINITY);
                     x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(FULL, x, 16));
@@ -480,8 +482,8 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             float w0[2], w1[2];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                w0[c] = fast_exp2(fmaf(s[nq][c], f0[nq][c], -m[nq][c]));
-                w1[c] = fast_exp2(fmaf(s[nq][2 + c], f1[nq][c], -m[nq][c]));
+                w0[c] = fast_exp2(__fadd_rn(s[nq][c], -m[nq][c]));
+                w1[c] = fast_exp2(__fadd_rn(s[nq][2 + c], -m[nq][c]));
             }
             if (valid < 16) {
                 if (g >= valid) w0[0] = w0[1] = 0.f;

@@ -241,9 +241,21 @@ __global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params
     }
 }
 
+// 16-bit values with NaN and infinities replaced by zero.
+template <typename T>
+__device__ __forceinline__ Vec16 finite8(Vec16 v) {
+    constexpr uint32_t top = Elem<T>::kUmmaFormat == 0 ? 0x7c00u : 0x7f80u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if ((v.w[i] & top) == top) v.w[i] &= 0xffff0000u;
+        if ((v.w[i] >> 16 & top) == top) v.w[i] &= 0xffffu;
+    }
+    return v;
+}
+
 // grid (logical pages, sequences).  Of several sequences that share a page the one that sees the most tokens (the later
-// one of equals) writes it, so no address has two writers.  Slots past its last token read as zero: what an earlier
-// owner of the page left there may be NaN, and the attention multiplies hidden values by zero.
+// one of equals) writes it.  Slots past its last token may hold anything an earlier owner of the page left, and the attention
+// multiplies hidden values by zero: what is not finite there is written as zero.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params p) {
     constexpr int LANES = D / 8;
@@ -264,7 +276,7 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
     const uint8_t* block = p.pool + p.layout.block_of(p.layer, page);
     const uint8_t* exps = block + 2 * p.layout.plane;
     T* image = reinterpret_cast<T*>(p.image) + (int64_t)page * rows * D;
-    const int total = rows * LANES;                                  // a multiple of 4 x 256 elements of 8 is the rule, not a must
+    const int total = rows * LANES;
     for (int i0 = threadIdx.x; i0 < total; i0 += kBatch8 * kThreads8) {
         uint2 q[kBatch8];
         uint8_t e[kBatch8];
@@ -273,7 +285,7 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
             const int i = i0 + u * kThreads8, r = i / LANES;
             q[u] = make_uint2(0u, 0u);
             e[u] = 0;
-            if (i < total && (visible == P || r % P < visible)) {
+            if (i < total) {
                 q[u] = __ldcs(reinterpret_cast<const uint2*>(block) + i);
                 e[u] = __ldg(exps + r);
             }
@@ -281,7 +293,10 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
 #pragma unroll
         for (int u = 0; u < kBatch8; u++) {
             const int i = i0 + u * kThreads8;
-            if (i < total) stg16(image + (int64_t)i * 8, expand8<T>(q[u], e[u]));
+            if (i >= total) continue;
+            Vec16 v = expand8<T>(q[u], e[u]);
+            if (visible < P && i / LANES % P >= visible) v = finite8<T>(v);
+            stg16(image + (int64_t)i * 8, v);
         }
     }
 }

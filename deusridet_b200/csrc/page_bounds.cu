@@ -189,23 +189,25 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// One warp walks pages of one (sequence, KV head), 8 to an int8 tile: the pages are its columns, the group's heads its rows.
-// Contraction order is free: a lane takes whole 16-byte chunks of a page's 2 D bound bytes, and the query bytes of the same
-// dims stay in registers over all pages.  The pass is bound by bytes in flight: bounds come by cp.async into a ring per warp,
-// 4 KB a stage, three stages ahead (held in registers, 4 to 8 KB a warp, 42 000 pages of 8 heads took 27-33 us).
+// One warp walks pages of one (sequence, KV head), 16 to an int8 tile: the pages are its rows, the group's heads its columns
+// (8 a tile), so that the maximum over the heads is two shuffles.  Contraction order is free: a lane takes whole 16-byte
+// chunks of a page's 2 D bound bytes, and the query bytes of the same dims stay in registers over all pages.  Bounds come by
+// cp.async into a ring per warp, 4 KB a stage at head_dim 128, three stages ahead.  42 000 pages of 8 heads (86 MB) take
+// 20 us; with heads as rows, their scales applied per page, and bounds held in registers 27 to 33 us.
 // The warps of a CTA take neighbouring heads of the same pages (their bounds lie side by side in memory), and where there
 // are fewer than four, stretches of the pages.  grid (page blocks, KV heads / heads_per_cta, sequences);
 // keys[(seq * Hkv + head) * stride + page].
-constexpr int kScoreWarps = 4, kScoreStages = 4, kScoreStageBytes = 4096;
+constexpr int kScoreWarps = 4, kScorePages = 16;                            // pages of a stage
+template <int D> constexpr int kScoreStages = D == 256 ? 3 : 4;
 template <typename T, int D, bool HI>
 __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const SelectParams p, int pages_per_cta, int heads_per_cta) {
     constexpr int CH = D / 64;                                              // query chunks (16 dims) a lane owns
-    constexpr int ROWB = 2 * D, CPR = ROWB / 16, SP = kScoreStageBytes / ROWB, TILES = SP / 8;   // pages and tiles of a stage
+    constexpr int ROWB = 2 * D, CPR = ROWB / 16, STAGE = kScorePages * ROWB, STAGES = kScoreStages<D>;
     constexpr int NR = HI ? 2 : 1;
     extern __shared__ __align__(128) uint8_t smem[];
     const int b = blockIdx.z, lane = threadIdx.x & 31, w = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int h = blockIdx.y * heads_per_cta + w % heads_per_cta, part = w / heads_per_cta, parts = kScoreWarps / heads_per_cta;
-    // lengths, rows, tables and bounds come from further back than the kernel directly in front, or from this library's
+    // lengths, rows and tables come from further back than the kernel directly in front
     const int row = __ldg(p.rows + b);
     const int len = min(__ldg(p.kv_len + b), p.max_kv_len);
     const int n = len <= 0 || row < 0 || row >= p.max_rows ? 0 : min((len - 1) / p.page_size + 1, p.table_stride);
@@ -233,27 +235,32 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
     };
     auto exponent_of = [&](int page) -> int { return page >= 0 ? __ldg(p.exponents + (layer0 + page) * p.num_kv_heads + h) : 0; };
     iss32 = checked(iss32);
-    int page32 = iss32, next32 = checked(iss_next);                         // of the window being scored, and the one behind it
+    iss_next = checked(iss_next);
+    int page32 = iss32, next32 = iss_next;                                  // of the window being scored, and the one behind it
     int e32 = exponent_of(page32), next_e = exponent_of(next32);
-    const uint32_t ring = smem_u32(smem) + w * kScoreStages * kScoreStageBytes;
-    const int n_stages = (last - begin + SP - 1) / SP;
+    const uint32_t ring = smem_u32(smem) + w * STAGES * STAGE;
+    const int n_stages = (last - begin + kScorePages - 1) / kScorePages;
+    // a lane's chunks of a stage are 32 apart: c = lane + 32 j, page c / CPR of the stage (see tile_off)
+    const int8_t* lane_src = p.bounds + (layer0 * p.num_kv_heads + h) * ROWB + 16 * (lane % CPR);
+    const uint32_t lane_dst = tile_off<ROWB>(lane / CPR, lane % CPR), page_bytes = (uint32_t)p.num_kv_heads * ROWB;
     auto issue = [&](int s) {
-        const int in_window = s * SP & 31;
-        if (in_window == 0 && s > 0) {
-            iss32 = checked(iss_next);
-            iss_next = page_ids(begin + s * SP + 32);
+        if ((s & 1) == 0 && s > 0) {
+            iss32 = iss_next;
+            iss_next = checked(page_ids(begin + s * kScorePages + 32));
         }
+        const uint32_t stage = ring + (s % STAGES) * STAGE;
 #pragma unroll
-        for (int j = 0; j < SP * CPR / 32; j++) {
-            const int c = lane + 32 * j, r = c / CPR, chunk = c % CPR;
-            const int page = __shfl_sync(FULL, iss32, in_window + r);       // the bounds of a hole are not read
-            copy16_or_zero(ring + (s % kScoreStages) * kScoreStageBytes + tile_off<ROWB>(r, chunk),
-                           p.bounds + ((layer0 + max(page, 0)) * p.num_kv_heads + h) * ROWB + 16 * chunk, page >= 0);
+        for (int j = 0; j < CPR / 2; j++) {
+            const int page = __shfl_sync(FULL, iss32, kScorePages * (s & 1) + lane / CPR + 32 * j / CPR);
+            constexpr int per = 32 / CPR > 0 ? 32 / CPR : 1;                // rows a step covers
+            const int row_j = per * j;
+            const uint32_t flip = tile_off<ROWB>(row_j, 0) & 127u, skip = tile_off<ROWB>(row_j, 0) & ~127u;
+            // the bounds of a hole are not read
+            copy16_or_zero(stage + (lane_dst ^ flip) + skip, lane_src + (uint64_t)(uint32_t)max(page, 0) * page_bytes, page >= 0);
         }
     };
     // ---- query rows, then the first bounds, then the query bytes ----
     uint32_t up[NR][CH][4], down[NR][CH][4];
-    int f[NR];
     Vec16 raw[NR][CH][2];
 #pragma unroll
     for (int r = 0; r < NR; r++)
@@ -266,14 +273,16 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
                     raw[r][i][c] = ldg16(reinterpret_cast<const T*>(p.q) + (((int64_t)b * p.num_kv_heads + h) * p.group + g + 8 * r) * D + 16 * (t + 4 * i) + 8 * c);
             }
 #pragma unroll
-    for (int s = 0; s < kScoreStages - 1; s++) {
+    for (int s = 0; s < STAGES - 1; s++) {
         if (s < n_stages) issue(s);
         copies_commit();
     }
+    int f_col[NR][2];                                                       // exponents of heads 2t and 2t + 1 (+ 8 r)
+    bool wide = false;                                                      // some head's exponent is far from fp32's middle
 #pragma unroll
     for (int r = 0; r < NR; r++) {
         float x[CH][16];
-        uint32_t amax = 0;
+        float top = 0.f;                                                    // NaN counts as nothing, here and below
 #pragma unroll
         for (int i = 0; i < CH; i++)
 #pragma unroll
@@ -281,77 +290,100 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
                 const float2 y = Elem<T>::unpack2(raw[r][i][j >> 2].w[j & 3]);
                 x[i][2 * j] = y.x;
                 x[i][2 * j + 1] = y.y;
-                // NaN counts as nothing, here and below
-                amax = max(amax, y.x == y.x ? __float_as_uint(y.x) & 0x7fffffffu : 0u);
-                amax = max(amax, y.y == y.y ? __float_as_uint(y.y) & 0x7fffffffu : 0u);
+                top = fmax3(top, fabsf(y.x), fabsf(y.y));
             }
+        uint32_t amax = __float_as_uint(top);
         amax = max(amax, __shfl_xor_sync(FULL, amax, 1));
         amax = max(amax, __shfl_xor_sync(FULL, amax, 2));
-        f[r] = bound_exponent(amax);
-        const float inv = exp2_int(-f[r]);
+        const int f = bound_exponent(amax);
+        const float inv = exp2_int(-f);
 #pragma unroll
         for (int i = 0; i < CH; i++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 uint32_t u = 0, d = 0;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float y = x[i][4 * k + j];
-                    const int v = y == y ? max(-127, min(127, __float2int_rn(fmaxf(-128.f, fminf(128.f, y * inv))))) : 0;
+                for (int j = 0; j < 4; j++) {                               // rounds to nearest even; NaN becomes 0, infinity 127
+                    const int v = max(-127, min(127, __float2int_rn(x[i][4 * k + j] * inv)));
                     u |= (uint32_t)(max(v, 0) & 0xff) << (8 * j);
                     d |= (uint32_t)(min(v, 0) & 0xff) << (8 * j);
                 }
                 up[r][i][k] = u;
                 down[r][i][k] = d;
             }
+        f_col[r][0] = __shfl_sync(FULL, f, 8 * t);                          // lane 4 (2t) holds head 2t's
+        f_col[r][1] = __shfl_sync(FULL, f, 8 * t + 4);
+        wide |= f > 60 || (f < -60 && amax != 0);
     }
+    wide = __any_sync(FULL, wide);
+    float scale[NR][2];                                                     // heads that are not there: -infinity by hand below
+#pragma unroll
+    for (int r = 0; r < NR; r++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) scale[r][c] = exp2_int(max(-126, f_col[r][c]));
     uint32_t* keys = p.keys + ((int64_t)b * p.num_kv_heads + h) * p.key_stride;
     uint32_t key = kKeyHole;                                                // of this lane's page of the window
     for (int s = 0; s < n_stages; s++) {
-        if (s + kScoreStages - 1 < n_stages) issue(s + kScoreStages - 1);
+        if (s + STAGES - 1 < n_stages) issue(s + STAGES - 1);
         copies_commit();
-        copies_wait<kScoreStages - 1>();
+        copies_wait<STAGES - 1>();
         __syncwarp();
-        const uint32_t stage = ring + (s % kScoreStages) * kScoreStageBytes;
-        const int in_window = s * SP & 31;
+        const uint32_t stage = ring + (s % STAGES) * STAGE;
+        int acc[NR][4] = {};
 #pragma unroll
-        for (int k = 0; k < TILES; k++) {
-            int acc[4] = {0, 0, 0, 0};
+        for (int i = 0; i < 2 * CH; i++) {                                  // upper bounds, then lower
+            const uint4 a = lds128(stage + tile_off<ROWB>(g, t + 4 * i)), c = lds128(stage + tile_off<ROWB>(g + 8, t + 4 * i));
 #pragma unroll
-            for (int i = 0; i < CH; i++) {
-                const uint4 hi4 = lds128(stage + tile_off<ROWB>(8 * k + g, t + 4 * i)), lo4 = lds128(stage + tile_off<ROWB>(8 * k + g, t + 4 * (CH + i)));
-                mma_s8(acc, up[0][i][0], HI ? up[NR - 1][i][0] : 0u, up[0][i][1], HI ? up[NR - 1][i][1] : 0u, hi4.x, hi4.y);
-                mma_s8(acc, up[0][i][2], HI ? up[NR - 1][i][2] : 0u, up[0][i][3], HI ? up[NR - 1][i][3] : 0u, hi4.z, hi4.w);
-                mma_s8(acc, down[0][i][0], HI ? down[NR - 1][i][0] : 0u, down[0][i][1], HI ? down[NR - 1][i][1] : 0u, lo4.x, lo4.y);
-                mma_s8(acc, down[0][i][2], HI ? down[NR - 1][i][2] : 0u, down[0][i][3], HI ? down[NR - 1][i][3] : 0u, lo4.z, lo4.w);
-            }
-            // heads g (and g + 8), pages in_window + 8 k + 2 t + c of the window
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const int e = __shfl_sync(FULL, e32, in_window + 8 * k + 2 * t + c);
-                float best = -INFINITY;
-#pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    const int ef = e + f[r], e1 = max(-126, min(127, ef));
-                    const float x = (float)acc[2 * r + c] * exp2_int(e1) * exp2_int(ef - e1);
-                    if (g + 8 * r < p.group) best = fmaxf(best, x);
-                }
-                best = fmaxf(best, __shfl_xor_sync(FULL, best, 4));
-                best = fmaxf(best, __shfl_xor_sync(FULL, best, 8));
-                best = fmaxf(best, __shfl_xor_sync(FULL, best, 16));
-                // to the lane whose page it is (every lane of a column holds it)
-                const float mine = __shfl_sync(FULL, best, (lane >> 1) & 3);
-                if (lane >> 3 == in_window / 8 + k && (lane & 1) == c) key = ordered(mine);
+            for (int r = 0; r < NR; r++) {
+                const uint32_t* q = i < CH ? up[r][i % CH] : down[r][i % CH];
+                mma_s8(acc[r], a.x, c.x, a.y, c.y, q[0], q[1]);
+                mma_s8(acc[r], a.z, c.z, a.w, c.w, q[2], q[3]);
             }
         }
         __syncwarp();                                                       // the stage is free for the next request
-        if (in_window + SP == 32 || s == n_stages - 1) {
-            const int idx = begin + (s * SP & ~31) + lane;
+        // pages g and g + 8 of the stage, heads 2t and 2t + 1 (+ 8 r)
+        float mine = 0.f;                                                   // of this lane's page, if it is in this stage
+        const int from = 4 * (lane & 7);                                    // a lane of that page's row of the tile
+        if (!wide) {
+            // whole number * 2^f is exact in fp32 here, and the maximum over the heads may come before 2^e
+            float best[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                float x = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        if (2 * t + c + 8 * r < p.group) x = fmaxf(x, (float)acc[r][2 * k + c] * scale[r][c]);
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 1));
+                best[k] = fmaxf(x, __shfl_xor_sync(FULL, x, 2));
+            }
+            const float b0 = __shfl_sync(FULL, best[0], from), b1 = __shfl_sync(FULL, best[1], from);
+            mine = ((lane & 8) ? b1 : b0) * exp2_int(e32);
+        } else {                                                            // the same in fp64, whose range holds every case
+            double best[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                double x = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        if (2 * t + c + 8 * r < p.group) x = fmax(x, ldexp((double)acc[r][2 * k + c], f_col[r][c]));
+                x = fmax(x, __shfl_xor_sync(FULL, x, 1));
+                best[k] = fmax(x, __shfl_xor_sync(FULL, x, 2));
+            }
+            const double b0 = __shfl_sync(FULL, best[0], from), b1 = __shfl_sync(FULL, best[1], from);
+            mine = (float)ldexp((lane & 8) ? b1 : b0, e32);
+        }
+        if (lane >> 4 == (s & 1)) key = ordered(mine);
+        if ((s & 1) || s == n_stages - 1) {                                 // a window of 32 pages is done
+            const int idx = begin + (s & ~1) * kScorePages + lane;
             if (idx < last)
                 keys[idx] = page32 < 0 ? kKeyHole : (idx < p.first_pages || idx >= n - p.last_pages) ? kKeyForced : key;
             page32 = next32;
             e32 = next_e;
-            next32 = checked(page_ids(begin + (s * SP & ~31) + 64));
+            next32 = checked(page_ids(begin + (s & ~1) * kScorePages + 64));
             next_e = exponent_of(next32);
         }
     }
@@ -532,7 +564,7 @@ cudaError_t launch_score(const SelectParams& p, int num_sms, cudaStream_t s) {
     const int64_t ctas = (int64_t)(p.num_kv_heads / heads) * p.n_seq;
     while (per_cta < 4096 && (pages + 2 * per_cta - 1) / (2 * per_cta) * ctas >= 9 * num_sms) per_cta *= 2;
     const dim3 grid((pages + per_cta - 1) / per_cta, p.num_kv_heads / heads, p.n_seq);
-    constexpr size_t smem = (size_t)kScoreWarps * kScoreStages * kScoreStageBytes;
+    constexpr size_t smem = (size_t)kScoreWarps * kScoreStages<D> * kScorePages * 2 * D;
     auto kernel = p.group > 8 ? page_score_kernel<T, D, true> : page_score_kernel<T, D, false>;
     static std::atomic<bool> configured[64][2];
     int dev = 0;

@@ -305,7 +305,8 @@ DRKV_API int drkv_select_pages(drkv_engine* e, int layer, int n_seq, const int32
 /* drkv_attend_decode over the listed pages only, of either kind of pool.  d_sel[n_seq][num_kv_heads][top_pages] need not come
  * from drkv_select_pages: of each list the first min(top_pages, ceil(kv_len / page_size)) entries are read; entries that are
  * negative, beyond the sequence or not resident contribute nothing, a page listed twice counts twice.  Keys at or
- * beyond kv_len are not seen.  Rows without any visible key are left as they are. */
+ * beyond kv_len are not seen.  Rows without any visible key are left as they are.  The importance scorer, if it is on,
+ * learns nothing from this call. */
 DRKV_API int drkv_attend_selected(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
                                   int max_kv_len, const int32_t* d_sel, int top_pages, const void* q, void* out, float scale,
                                   void* stream);

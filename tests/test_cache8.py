@@ -416,6 +416,60 @@ def test_prefill_over_the_pool(drkv_lib, dtype, d, grp, page):
 
 
 @pytest.mark.gpu
+def test_prefill_pages_shared_out_of_step(drkv_lib):
+    """One page at different places of two sequences' tables, whole for one and the tail of the other, in one call."""
+    import torch
+    eng = _engine(hq=4, hkv=1, d=64, page=16, dtype="bf16", pages=8, seqs=3, per_seq=4)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, 48)
+    eng.set_seq_len(0, 48)
+    eng.sync_block_table()
+    stored = _fill(eng, [48], "bf16", 1, spread=1)[0]
+    other = eng.seq_create()
+    pages = [int(p) for p in eng.table(0)[:3]]
+    eng.adopt(other, [pages[2], pages[0]], 20)                       # its last page holds 4 tokens of the parent's first 16
+    eng.sync_block_table()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qs = [torch.randn(4, 4, 64, generator=g, device="cuda").bfloat16() for _ in range(2)]
+    outs = [torch.zeros_like(q) for q in qs]
+    eng.attend_prefill_batch(0, [0, other], [44, 16], [4, 4], qs, outs, 0.125)
+    torch.cuda.synchronize()
+    order = [np.arange(48), np.concatenate([np.arange(32, 48), np.arange(16)])]
+    for i, start in enumerate((44, 16)):
+        for t in range(4):
+            see = order[i][:start + t + 1]
+            want, pv, mag = R.attend(qs[i][t].double().cpu().numpy(), stored[0][see, 0], stored[1][see, 0], 0.125)
+            tol = R.attend_tolerance(want, pv, mag, _half_step("bf16"), _half_step("bf16"))
+            assert (np.abs(outs[i][t].double().cpu().numpy() - want) <= tol).all(), (i, t)
+    eng.close()
+
+
+@pytest.mark.gpu
+def test_more_sequences_than_one_launch(drkv_lib):
+    """1030 rows of a batch over three sequences: two launches, every row as a batch of one gives it but for the split."""
+    import torch
+    lens = [40, 7, 100]
+    eng = _engine(hq=4, hkv=2, d=64, page=16, dtype="f16", pages=16, seqs=3, per_seq=8)
+    for s, n in enumerate(lens):
+        eng.seq_create()
+        assert eng.ensure_blocks_for_range(s, 0, n)
+        eng.set_seq_len(s, n)
+    eng.sync_block_table()
+    stored = _fill(eng, lens, "f16", 1)
+    n = 1030
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn(n, 4, 64, generator=g, device="cuda").half()
+    rows = torch.arange(n, device="cuda", dtype=torch.int32) % 3
+    kv_len = torch.tensor(lens, device="cuda", dtype=torch.int32)[rows.long()].contiguous()
+    out = torch.zeros_like(q)
+    eng.attend_decode(0, n, rows, kv_len, 100, q, out, 0.1)
+    torch.cuda.synchronize()
+    some = [0, 1, 2, 500, 1021, 1022, 1023, 1024, 1025, 1026, 1029]
+    _check_decode(out[some], out[some], q[some], [stored[i % 3] for i in some], [lens[i % 3] for i in some], 2, 0.1, "f16")
+    eng.close()
+
+
+@pytest.mark.gpu
 def test_fork_copy_on_write_and_tier(drkv_lib, tmp_path):
     """A fork's write leaves the parent's page alone; pages that went to files and back hold the same bytes."""
     import torch

@@ -192,6 +192,9 @@ def test_select_and_attend(drkv_lib, pool, dtype, d, grp, hkv, page):
     eng.sync_block_table()
     q = torch.randn(len(lens), grp * hkv, d, generator=g, device="cuda").to(t)
     q[6] *= 1e-3
+    if dtype == "bf16":                                             # exponents at the ends of fp32, heads far apart
+        q[4, 0], q[4, -1] = q[4, 0] * 1e-25, q[4, -1] * 1e-36
+        q[7] *= 1e25
     rows = torch.arange(len(lens), device="cuda", dtype=torch.int32)
     kv_len = torch.tensor(lens, device="cuda", dtype=torch.int32)
     scale = 1.0 / math.sqrt(d)
