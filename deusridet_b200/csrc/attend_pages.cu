@@ -5,11 +5,14 @@
 // 4 D flops per key and query head ride on mma.sync tiles far from their limit (a GQA group fills one 8-column tile).
 //
 // Split: the keys of all (sequence, KV head) pairs form one line of 16-key groups.  Every warp of a persistent grid takes
-// an equal stretch of it, whatever the lengths are: ragged batches need no queue and no tail, and short lines (one group a
-// warp: 11.3 us for 1500 keys; four: 14.0) are spread as far as they go.  A pair that lies inside one stretch is finished by its warp; one that is cut leaves a piece (m, l, o) per stretch,
-// at most two a warp, and a second small kernel merges them in a fixed order (results do not depend on timing).  Warps of
-// one CTA take stretches far apart, so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and
-// then by the last CTA to arrive, took 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end.
+// an equal stretch of it, whatever the lengths are: ragged batches need no queue and no tail, and short lines are spread as
+// far as they go (1500 keys of 4 heads: 11.3 us a step with one group a warp, 14.0 with four).  A pair that lies inside one
+// stretch is finished by its warp; one that is cut leaves a piece (m, l, o) per stretch, at most two a warp, and a second
+// small kernel merges them in a fixed order (results do not depend on timing).  Warps of one CTA take stretches far apart,
+// so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and then by the last CTA to arrive, took
+// 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end.
+// Bound by HBM: the loop over groups reads 7 TB/s (131 001 keys of 8 heads, 270 MB: 50 us, 8 more for the merge; 64 sequences
+// of 1-8 k keys, 602 MB: 106 us); what is left is the first data of a launch, the uneven finish and the merge.
 //
 // A warp brings its groups into a private ring of shared memory by cp.async (16 bytes a lane, L1 bypassed), kStages - 1
 // groups ahead, and reads them as matrix operands without ldmatrix: contraction order is free, so a lane takes whole
@@ -19,7 +22,8 @@
 // become f16 two at a time (cvt.rn.f16x2.e4m3x2, exact).
 //
 // Scales of the 8-bit rows stay exponents.  K's multiply the score.  V's multiply the weight: with E the largest exponent
-// seen so far, weights are p * 2^(ev - E + 15) <= 2^15 in f16, full precision down to 2^-29 of the largest; o carries 2^E.
+// seen so far, weights are p * 2^(ev - E + 7) in f16, at most 2^15 since p may reach 2^8 before the maximum follows, and of
+// full precision down to 2^-21 of the largest; o carries 2^E.
 // bf16 queries are scaled by a power of two per head into f16 (8 significant bits fit; exact unless an element is below
 // 2^-27 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
 // P in the PV product: f16 hi + lo terms (22 bits) where the output is f16, bf16 hi + lo (16 bits) for a bf16 pool,

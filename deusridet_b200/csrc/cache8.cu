@@ -20,10 +20,6 @@ constexpr int kThreads8 = 256;
 constexpr int kMaxTokens8 = 32;   // tokens of one CTA of the append
 constexpr int kBatch8 = 4;        // rows a lane has in flight
 
-// n / d for n * d < 2^32 by a multiplication; magic 0 stands for d = 1.
-__host__ __device__ __forceinline__ uint32_t magic_of(uint32_t d) { return d <= 1 ? 0 : (uint32_t)((0x100000000ull + d - 1) / d); }
-__device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t magic) { return magic ? __umulhi(n, magic) : n; }
-
 // Quantises the row of which each of its LANES lanes holds 8 elements; row: its index in the block's rows (K plane, then V
 // plane, exponents in the same order).
 template <int LANES>

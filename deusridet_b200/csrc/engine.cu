@@ -223,6 +223,11 @@ static constexpr size_t kPlanInts = (size_t)kMaxDecodeSeqs * 3 + (size_t)kMaxDec
         if (ce_ != cudaSuccess) return set_err(DRKV_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(ce_)); \
     } while (0)
 
+// Rows that kernels read or write in 16-byte vectors.
+static bool aligned16(const void* a, const void* b = nullptr) {
+    return (reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) % 16 == 0;
+}
+
 static int book_err(drkv_engine* e, int rc) {
     if (rc < 0) g_err = e->book.error();
     return rc;
@@ -846,6 +851,7 @@ static AppendParams append_params(drkv_engine* e, int layer) {
 
 static int append8(drkv_engine* e, int layer, int n, const int32_t* d_rows, const int32_t* d_pos, int row, int pos_start,
                    const void* k_src, const void* v_src, cudaStream_t stream) {
+    if (!aligned16(k_src, v_src)) return set_err(DRKV_ERR_INVALID, "append: K and V sources must be 16-byte aligned");
     Append8Params p{};
     p.layout = e->layout8;
     p.pool = static_cast<uint8_t*>(e->pool);
@@ -919,6 +925,7 @@ static int seq_flat_copy(drkv_engine* e, int seq, int start_token, int num_token
         return set_err(DRKV_ERR_INVALID, "extract/inject: bad argument");
     if (num_tokens > INT32_MAX - start_token) return set_err(DRKV_ERR_INVALID, "extract/inject: positions beyond 2^31");
     if (e->pool8) {
+        if (!aligned16(flat)) return set_err(DRKV_ERR_INVALID, "extract/inject: the flat buffer must be 16-byte aligned");
         DeviceGuard dev(e->device);
         note_stream(e, (cudaStream_t)stream);
         Flat8Params f{};
@@ -1112,6 +1119,7 @@ static int decode_common(drkv_engine* e, int layer, int n_seq, const int32_t* d_
 static int attend_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
                         const int32_t* d_list, int list_len, const void* q, void* out, float scale, cudaStream_t stream) {
     const drkv_geometry& g = e->geom;
+    if (!aligned16(q, out)) return set_err(DRKV_ERR_INVALID, "attend: q and out must be 16-byte aligned");
     DeviceGuard dev(e->device);
     note_stream(e, stream);
     const int64_t row_tokens = (int64_t)e->book.row_width() * g.page_size;
@@ -1911,6 +1919,7 @@ int drkv_select_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_row
         return set_err(DRKV_ERR_INVALID, "select_pages: bad argument");
     if (top_pages < 1 || first_pages < 0 || last_pages < 0 || (int64_t)first_pages + last_pages > top_pages)
         return set_err(DRKV_ERR_INVALID, "select_pages: top_pages must be positive and hold first_pages + last_pages");
+    if (!aligned16(q)) return set_err(DRKV_ERR_INVALID, "select_pages: q must be 16-byte aligned");
     if (!e->bounds.on) return set_err(DRKV_ERR_STATE, "select_pages: page bounds are not enabled");
     if (n_seq == 0) return DRKV_OK;
     DeviceGuard dev(e->device);

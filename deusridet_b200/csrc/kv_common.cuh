@@ -172,6 +172,10 @@ __device__ __forceinline__ void rope_pair(float x0, float x1, float c, float s, 
     y1 = __fmaf_rn(x1, c, __fmul_rn(x0, s));
 }
 
+// n / d for n * d < 2^32 by a multiplication; magic 0 stands for d = 1.
+__host__ __device__ __forceinline__ uint32_t magic_of(uint32_t d) { return d <= 1 ? 0 : (uint32_t)((0x100000000ull + d - 1) / d); }
+__device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t magic) { return magic ? __umulhi(n, magic) : n; }
+
 struct alignas(16) Vec16 {
     uint32_t w[4];
 };

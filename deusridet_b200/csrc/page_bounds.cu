@@ -9,8 +9,8 @@
 // order and on every unit, so equal scores are equal bits and the selection is reproducible (ties: lowest page).
 // As a contraction: [q8 clipped to >= 0, q8 clipped to <= 0] . [b_max, b_min], 2 D long, on int8 mma.sync tiles.
 //
-// The score pass reads (2 D + 1) bytes per page and KV head, D + 1/2 times fewer than 2 P rows of 16 bits would be: HBM-
-// bound for long contexts; the selection runs on the scores in shared memory, one CTA per (sequence, KV head).
+// The score pass reads 2 D + 1 bytes per page and KV head where the page's K and V rows are 4 P D in 16 bits: HBM-bound for
+// long contexts; the selection runs on the scores in shared memory, one CTA per (sequence, KV head).
 #include <atomic>
 
 #include "kernels.hpp"

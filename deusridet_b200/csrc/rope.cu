@@ -52,10 +52,8 @@ struct RopeParams {
     // items of one (token, head) row: rot_items of VW pairs each, then copy_items of VW elements each (rows that
     // are not rotated in place)
     int rot_items, row_items;
-    uint32_t magic_row, magic_heads; // ceil(2^32 / divisor): n / divisor for n * divisor < 2^32; 0 stands for divisor 1
+    uint32_t magic_row, magic_heads; // of row_items and heads, see div_magic
 };
-
-__device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t magic) { return magic ? __umulhi(n, magic) : n; }
 
 // Cosines and sines of a CTA's tokens, one per thread.
 __device__ __forceinline__ void fill_trig(const RopeParams& p, float* s_trig, int tok0, int n_tok, int pad) {
@@ -239,8 +237,6 @@ int fail(int code, const char* msg) {
     return code;
 }
 
-uint32_t magic_of(uint32_t d) { return d <= 1 ? 0 : (uint32_t)((0x100000000ull + d - 1) / d); }
-
 // Largest vector width the rows allow: every address they form is a multiple of it.
 int widest(const drkv_rope_rows& r, int n_tokens, int vw) {
     auto fits = [&](const void* ptr, int64_t tok, int64_t head) {
@@ -349,14 +345,20 @@ int drkv_rope_create(const drkv_rope_config* cfg, drkv_rope** out) {
     r->factor = c.attention_factor > 0.f ? c.attention_factor
                 : c.scaling == DRKV_ROPE_RAMP ? (float)(0.1 * log(c.factor) + 1.0)
                                               : 1.f;
-    std::vector<long double> f;
-    frequencies(c, &f);
-    std::vector<uint64_t> turns(f.size());
-    for (size_t i = 0; i < f.size(); i++) {
-        r->freq.push_back((double)f[i]);
-        const long double t = f[i] / (2 * 3.141592653589793238462643383279502884L);
-        const long double frac = t - floorl(t);
-        turns[i] = frac >= 1.0L ? 0 : (uint64_t)ldexpl(frac, 64);
+    std::vector<uint64_t> turns;
+    try {
+        std::vector<long double> f;
+        frequencies(c, &f);
+        turns.resize(f.size());
+        for (size_t i = 0; i < f.size(); i++) {
+            r->freq.push_back((double)f[i]);
+            const long double t = f[i] / (2 * 3.141592653589793238462643383279502884L);
+            const long double frac = t - floorl(t);
+            turns[i] = frac >= 1.0L ? 0 : (uint64_t)ldexpl(frac, 64);
+        }
+    } catch (const std::bad_alloc&) {
+        delete r;
+        return fail(DRKV_ERR_CAPACITY, "rope_create: out of host memory");
     }
     if (c.device >= 0) {
         DeviceGuard dev(c.device);
@@ -434,7 +436,7 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
     }
     const int qh = q ? q->heads : 0, kh = k ? k->heads : 0;
     if (n_tokens == 0 || qh + kh == 0) return DRKV_OK;
-    if (!d_pos) return fail(DRKV_ERR_INVALID, "rope_apply: null positions");
+    if (!d_pos || reinterpret_cast<uintptr_t>(d_pos) % 4) return fail(DRKV_ERR_INVALID, "rope_apply: null or unaligned positions");
     RopeParams p{};
     auto rows = [](const drkv_rope_rows& x) {
         return RopeRowsDev{x.src, x.dst, x.src_token_stride, x.src_head_stride, x.dst_token_stride, x.dst_head_stride};

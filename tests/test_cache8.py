@@ -519,7 +519,10 @@ def test_refusals_on_device(drkv_lib):
     for call in (lambda: eng.attend_partial(0, 0, 0, 4, x, part, 1.0), lambda: eng.exchange_create(2, 0),
                  lambda: eng.append_rope_chunk(0, 0, 2 ** 31 - 4, 16, x, x), lambda: eng.extract(0, 2 ** 31 - 4, 16, x),
                  lambda: eng.append_rope(1, 1, one, one, x, x), lambda: eng.attend_decode(0, 1, one, one, -1, x, x, 1.0),
-                 lambda: eng.append_rope_chunk(0, 1, 0, 1, x, x)):
+                 lambda: eng.append_rope_chunk(0, 1, 0, 1, x, x), lambda: eng.append_rope_chunk(0, 0, 0, 1, x.data_ptr() + 2, x),
+                 lambda: eng.append_rope(0, 1, one, one, x, x.data_ptr() + 8), lambda: eng.extract(0, 0, 1, x.data_ptr() + 8),
+                 lambda: eng.inject(0, 0, 1, x.data_ptr() + 2), lambda: eng.attend_decode(0, 1, one, one, 16, x.data_ptr() + 2, x, 1.0),
+                 lambda: eng.append_attend_decode(0, 1, one, one, 16, x, x, x, x.data_ptr() + 4, 1.0)):
         with pytest.raises(DrkvError) as err:
             call()
         assert err.value.code == capi.ERR_INVALID

@@ -314,6 +314,9 @@ def test_refusals(drkv_lib):
                  lambda: eng.select_pages(0, 1, one, one, 16, x, 4, 3, 2, sel), lambda: eng.select_pages(0, 1, one, one, 16, x, 4, -1, 2, sel),
                  lambda: eng.select_pages(0, 1, one, one, 16, x, 2, 2 ** 31 - 1, 2 ** 31 - 1, sel),
                  lambda: eng.select_pages(0, 1, one, one, -1, x, 4, 1, 1, sel), lambda: eng.select_pages(0, 1, one, one, 16, None, 4, 1, 1, sel),
+                 lambda: eng.select_pages(0, 1, one, one, 16, x.data_ptr() + 2, 4, 1, 1, sel),
+                 lambda: eng.attend_selected(0, 1, one, one, 16, sel, 4, x.data_ptr() + 2, x, 1.0),
+                 lambda: eng.attend_selected(0, 1, one, one, 16, sel, 4, x, x.data_ptr() + 8, 1.0),
                  lambda: eng.attend_selected(0, 1, one, one, 16, None, 4, x, x, 1.0),
                  lambda: eng.attend_selected(0, 1, one, one, 16, sel, 0, x, x, 1.0), lambda: eng.attend_selected(0, -1, one, one, 16, sel, 4, x, x, 1.0)):
         with pytest.raises(DrkvError) as err:
