@@ -44,7 +44,7 @@ constexpr float kNoKey = -3.402823466e38f;   // running maximum before any key: 
 // Warps per CTA (one CTA per SM) and groups in a warp's ring.
 template <bool POOL8, int D, int NQ> struct Ring;
 template <int NQ> struct Ring<true, 64, NQ>   { static constexpr int kWarps = 16, kStages = 4; };   // 132 KB
-template <> struct Ring<true, 128, 1>         { static constexpr int kWarps = 16, kStages = 3; };   // 198 KB
+template <> struct Ring<true, 128, 1>         { static constexpr int kWarps = 12, kStages = 4; };   // 198 KB
 template <> struct Ring<true, 128, 2>         { static constexpr int kWarps = 12, kStages = 4; };   // 198 KB
 template <int NQ> struct Ring<true, 256, NQ>  { static constexpr int kWarps = 8, kStages = 3; };    // 197 KB
 template <int NQ> struct Ring<false, 64, NQ>  { static constexpr int kWarps = 16, kStages = 3; };   // 192 KB
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
 // PARTS-th piece, eight pieces' loads in flight at a time: the kernel is a chain of L2 latencies.  CTA_DIMS == 0: many rows of a
 // few pieces, one set a row.  CTA_DIMS > 0: a CTA takes that many of one row with as many sets as fit.
 template <typename T, int D, int CTA_DIMS>
-__global__ void __launch_bounds__(CTA_DIMS ? 256 : 128) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
+__global__ void __launch_bounds__(CTA_DIMS ? 256 : 128, 1) merge_pieces_kernel(const AttendPagesParams p, int n_warps) {
     constexpr bool WIDE = CTA_DIMS > 0;
     constexpr int DIMS = WIDE ? CTA_DIMS : D, LANES = DIMS / 4;
     constexpr int PARTS = WIDE ? 256 / LANES : 1, ROWS = WIDE ? 1 : 128 / LANES;
