@@ -301,13 +301,18 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
         for (int i = 0; i < CH; i++)
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                uint32_t u = 0, d = 0;
+                // adding 1.5 * 2^23 rounds to the nearest even whole number and leaves it in the low byte; NaN becomes 0,
+                // infinity 127
+                constexpr float magic = 12582912.f;
+                uint32_t ub[4], db[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {                               // rounds to nearest even; NaN becomes 0, infinity 127
-                    const int v = max(-127, min(127, __float2int_rn(x[i][4 * k + j] * inv)));
-                    u |= (uint32_t)(max(v, 0) & 0xff) << (8 * j);
-                    d |= (uint32_t)(min(v, 0) & 0xff) << (8 * j);
+                for (int j = 0; j < 4; j++) {
+                    const float y = x[i][4 * k + j] * inv;
+                    ub[j] = __float_as_uint(fminf(fmaxf(y, 0.f), 127.f) + magic);
+                    db[j] = __float_as_uint(fmaxf(fminf(y, 0.f), -127.f) + magic);
                 }
+                const uint32_t u = __byte_perm(__byte_perm(ub[0], ub[1], 0x0040), __byte_perm(ub[2], ub[3], 0x0040), 0x5410);
+                const uint32_t d = __byte_perm(__byte_perm(db[0], db[1], 0x0040), __byte_perm(db[2], db[3], 0x0040), 0x5410);
                 up[r][i][k] = u;
                 down[r][i][k] = d;
             }
