@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
     const int lanes = 1 << lanes_log2, l = threadIdx.x & (lanes - 1), rows_at_once = kRopeThreads >> lanes_log2;
     const int total = n_tok * p.heads, rot_lanes = (p.rotary_dim + 7) >> 3, half_lanes = half >> 3;
     const bool turns = l < rot_lanes;
+    const int live_pairs = half - 4 * l;                        // pairs layout: of the lane's four, those that turn
     const bool second = !PAIRS && l >= half_lanes;
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
     const int trig0 = turns ? (PAIRS ? 4 * l : 8 * (second ? l - half_lanes : l)) : 0;
@@ -214,8 +215,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
                 y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, second ? s[2 * i] : -s[2 * i]));
                 y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, second ? s[2 * i + 1] : -s[2 * i + 1]));
             }
-            // (pairs: the last vector that turns may hold pairs that do not)
-            y.w[i] = turns && (!PAIRS || 4 * l + i < half) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
+            y.w[i] = (PAIRS ? i < live_pairs : turns) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
         }
         if (x.dst != nullptr) stg16(x.dst, y);
     };
