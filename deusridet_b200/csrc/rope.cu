@@ -46,26 +46,36 @@ struct RopeParams {
     const int32_t* pos;
     const uint64_t* turns;
     int n_tokens, q_heads, heads;    // heads = query heads + key heads
-    int half, rotary_dim, tokens_per_cta;
+    int half, rotary_dim, tokens_per_cta, heads_per_cta;
     int pairs_layout, inverse;
     float factor;
     // items of one (token, head) row: rot_items of VW pairs each, then copy_items of VW elements each (rows that
     // are not rotated in place)
     int rot_items, row_items;
-    uint32_t magic_row, magic_heads; // of row_items and heads, see div_magic
+    uint32_t magic_row, magic_heads; // of row_items and heads_per_cta, see div_magic
 };
 
-// Cosines and sines of a CTA's tokens, one per thread.
+// Cosines and sines of a CTA's tokens, one pair per thread: [token][cosines | sines][pad].  PER_DIM: one of each for every
+// dim that turns, the sine with the sign that the dim's own formula gives it.
+template <bool PER_DIM>
 __device__ __forceinline__ void fill_trig(const RopeParams& p, float* s_trig, int tok0, int n_tok, int pad) {
-    for (int i = threadIdx.x; i < n_tok * pad; i += kRopeThreads) {
-        const int t = i / pad, j = i - t * pad;
+    const int n = PER_DIM ? p.half : pad;
+    for (int i = threadIdx.x; i < n_tok * n; i += kRopeThreads) {
+        const int t = i / n, j = i - t * n;
         if (j < p.half) {
             const uint64_t phase = (uint64_t)(int64_t)__ldg(p.pos + tok0 + t) * __ldg(p.turns + j);
             const int hi = (int)(uint32_t)((phase + 0x80000000ull) >> 32);
             float s, c;
             sincospif((float)hi * 0x1p-31f, &s, &c);
-            s_trig[t * 2 * pad + j] = c * p.factor;
-            s_trig[t * 2 * pad + pad + j] = (p.inverse ? -s : s) * p.factor;
+            c *= p.factor;
+            s = (p.inverse ? -s : s) * p.factor;
+            float* to = s_trig + t * 2 * pad + j;
+            to[0] = c;
+            to[pad] = PER_DIM ? -s : s;
+            if (PER_DIM) {
+                to[p.half] = c;
+                to[pad + p.half] = s;
+            }
         }
     }
 }
@@ -79,7 +89,7 @@ template <> struct RopeVec<1> { using type = uint16_t; };
 // A thread takes items of VW pairs (two vectors of VW elements).  VW is the widest of 8, 4, 2, 1 that divides half the
 // rotated dims and every stride and alignment; 16-byte vectors for the usual heads, 2-byte ones only for odd halves.
 // tokens_per_cta tokens share a CTA: their cosines and sines are evaluated once into shared memory, one per thread,
-// and used by every head.
+// and used by every head (blockIdx.y: a share of the heads, while there are few tokens).
 template <typename T, int VW>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
     extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][half_pad]
@@ -89,9 +99,9 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
     const int half = p.half, pad = (half + 3) & ~3;
     const int tok0 = blockIdx.x * p.tokens_per_cta;
     const int n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
-    fill_trig(p, s_trig, tok0, n_tok, pad);
+    fill_trig<false>(p, s_trig, tok0, n_tok, pad);
     __syncthreads();
-    const uint32_t per_token = (uint32_t)p.heads * p.row_items, total = per_token * n_tok;
+    const uint32_t per_token = (uint32_t)p.heads_per_cta * p.row_items, total = per_token * n_tok;
     for (uint32_t base = threadIdx.x; base < total; base += kRopeThreads * kRopeUnroll) {
         V a[kRopeUnroll], b[kRopeUnroll];
         T* dst[kRopeUnroll];
@@ -103,7 +113,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
             trig[u] = -1;
             if (it >= total) continue;
             const uint32_t row = div_magic(it, p.magic_row), j = it - row * p.row_items;
-            const uint32_t t = div_magic(row, p.magic_heads), h = row - t * p.heads;
+            const uint32_t t = div_magic(row, p.magic_heads), h = row - t * p.heads_per_cta + blockIdx.y * p.heads_per_cta;
+            if ((int)h >= p.heads) continue;
             const bool is_k = (int)h >= p.q_heads;
             const RopeRowsDev& r = is_k ? p.k : p.q;
             const int64_t head = is_k ? (int)h - p.q_heads : (int)h, tok = tok0 + (int)t;
@@ -162,20 +173,31 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 // that 2 048 threads an SM keep loads in flight: 32 768 tokens of 40 heads of 128 122 us (5.5 TB/s); four rows a lane at 80
 // registers: 138.
 // (The general kernel above loses on them by index arithmetic per vector: 158 us.)
-template <typename T, bool PAIRS>
-__global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopeParams p, int lanes_log2) {
-    extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][half_pad]
+// Halves of a width that is no multiple of 8 (kAnyHalves): a lane's partners lie across two vectors, so a warp lays the row
+// into shared memory as a ring (the first half once more behind the second), where the partner of dim e is at e + half
+// (50 of 64 dims of 28 heads, 7 401 tokens: 20 us; the general kernel, by single elements, 36).
+enum RopeMode { kHalves, kPairs, kAnyHalves };
+
+// Elements of a row's ring: rotary_dim + half, and what a lane reads past its own.
+__host__ __device__ constexpr int ring_elements(int lanes) { return 12 * lanes + 16; }
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 5 : 8) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+    constexpr bool PAIRS = MODE == kPairs, ANY = MODE == kAnyHalves;
+    extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][pad], then the rows' rings
     pdl_wait();
     pdl_launch_dependents();
-    const int half = p.half, pad = (half + 3) & ~3;
+    const int half = p.half, pad = ANY ? (p.rotary_dim + 7) & ~7 : (half + 3) & ~3;
     const int tok0 = blockIdx.x * p.tokens_per_cta, n_tok = min(p.tokens_per_cta, p.n_tokens - tok0);
     const int lanes = 1 << lanes_log2, l = threadIdx.x & (lanes - 1), rows_at_once = kRopeThreads >> lanes_log2;
-    const int total = n_tok * p.heads, rot_lanes = (p.rotary_dim + 7) >> 3, half_lanes = half >> 3;
+    const int total = n_tok * p.heads_per_cta, rot_lanes = (p.rotary_dim + 7) >> 3, half_lanes = half >> 3;
     const bool turns = l < rot_lanes;
-    const int live_pairs = half - 4 * l;                        // pairs layout: of the lane's four, those that turn
+    const int live_pairs = half - 4 * l;                        // of the lane's four words, those that turn (not kHalves)
     const bool second = !PAIRS && l >= half_lanes;
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
-    const int trig0 = turns ? (PAIRS ? 4 * l : 8 * (second ? l - half_lanes : l)) : 0;
+    const int trig0 = !turns ? 0 : PAIRS ? 4 * l : ANY ? 8 * l : 8 * (second ? l - half_lanes : l);
+    const int ring = ring_elements(lanes);
+    uint32_t* row_ring = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(s_trig + p.tokens_per_cta * 2 * pad) + (threadIdx.x >> lanes_log2) * ring);
     struct Row {
         Vec16 v;
         T* dst;                                                 // null: nothing to write
@@ -184,7 +206,8 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
     auto read = [&](int row) -> Row {
         Row x{Vec16{{0u, 0u, 0u, 0u}}, nullptr, 0};
         if (row >= total) return x;
-        const int t = div_magic(row, p.magic_heads), h = row - t * p.heads;
+        const int t = div_magic(row, p.magic_heads), h = row + ((int)blockIdx.y - t) * p.heads_per_cta;
+        if (h >= p.heads) return x;
         const bool is_k = h >= p.q_heads;
         const RopeRowsDev& r = is_k ? p.k : p.q;
         if (!turns && r.src == r.dst) return x;                 // in place, and these dims stay
@@ -202,26 +225,44 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_rows_kernel(const RopePa
             *reinterpret_cast<float4*>(c + 4 * i) = cs[i];
             *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + i];
         }
-        Vec16 y;
+        Vec16 y, other = x.v;
+        if (ANY) {
+            __syncwarp();                                       // the row before has been read
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i < live_pairs) row_ring[4 * l + i] = x.v.w[i];
+                if (8 * l + 2 * i < half) row_ring[half + 4 * l + i] = x.v.w[i];
+            }
+            __syncwarp();
+            if (turns) {
+                const uint32_t* from = row_ring + ((8 * l + half) >> 1);
+#pragma unroll
+                for (int i = 0; i < 4; i++) other.w[i] = __funnelshift_r(from[i], from[i + 1], half & 1 ? 16 : 0);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float2 own = Elem<T>::unpack2(x.v.w[i]);
             float y0, y1;
             if (PAIRS) {
                 rope_pair(own.x, own.y, c[i], s[i], y0, y1);
+            } else if (ANY) {
+                const float2 o = Elem<T>::unpack2(other.w[i]);
+                y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, s[2 * i]));
+                y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, s[2 * i + 1]));
             } else {
                 const float2 o = Elem<T>::unpack2(__shfl_sync(0xffffffffu, x.v.w[i], partner));
                 // first half: x0 c - x1 s; second: x1 c + x0 s
                 y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, second ? s[2 * i] : -s[2 * i]));
                 y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, second ? s[2 * i + 1] : -s[2 * i + 1]));
             }
-            y.w[i] = (PAIRS ? i < live_pairs : turns) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
+            y.w[i] = (MODE == kHalves ? turns : i < live_pairs) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
         }
         if (x.dst != nullptr) stg16(x.dst, y);
     };
     const int r_own = threadIdx.x >> lanes_log2;
     Row a = read(r_own), b;                                     // on its way while the cosines are evaluated
-    fill_trig(p, s_trig, tok0, n_tok, pad);
+    fill_trig<ANY>(p, s_trig, tok0, n_tok, pad);
     __syncthreads();
     for (int r0 = 0; r0 < total; r0 += 2 * rows_at_once) {      // the whole CTA together: rows r0 + r_own, then the next
         b = read(r0 + rows_at_once + r_own);
@@ -259,12 +300,21 @@ bool rows_apart(int64_t tok, int64_t head, int n_tokens, int heads, int d) {
 }
 
 template <typename T>
-cudaError_t launch_rope(const RopeParams& p, int vw, int grid, size_t smem, cudaStream_t stream) {
+cudaError_t launch_rope(const RopeParams& p, int vw, dim3 grid, size_t smem, cudaStream_t stream) {
     switch (vw) {
-        case 8: return launch_pdl(rope_kernel<T, 8>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
-        case 4: return launch_pdl(rope_kernel<T, 4>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
-        case 2: return launch_pdl(rope_kernel<T, 2>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
-        default: return launch_pdl(rope_kernel<T, 1>, dim3(grid), dim3(kRopeThreads), smem, stream, p);
+        case 8: return launch_pdl(rope_kernel<T, 8>, grid, dim3(kRopeThreads), smem, stream, p);
+        case 4: return launch_pdl(rope_kernel<T, 4>, grid, dim3(kRopeThreads), smem, stream, p);
+        case 2: return launch_pdl(rope_kernel<T, 2>, grid, dim3(kRopeThreads), smem, stream, p);
+        default: return launch_pdl(rope_kernel<T, 1>, grid, dim3(kRopeThreads), smem, stream, p);
+    }
+}
+
+template <typename T>
+cudaError_t launch_rows(const RopeParams& p, int mode, int lg, dim3 grid, size_t smem, cudaStream_t stream) {
+    switch (mode) {
+        case kPairs: return launch_pdl(rope_rows_kernel<T, kPairs>, grid, dim3(kRopeThreads), smem, stream, p, lg);
+        case kHalves: return launch_pdl(rope_rows_kernel<T, kHalves>, grid, dim3(kRopeThreads), smem, stream, p, lg);
+        default: return launch_pdl(rope_rows_kernel<T, kAnyHalves>, grid, dim3(kRopeThreads), smem, stream, p, lg);
     }
 }
 
@@ -456,24 +506,31 @@ int drkv_rope_apply(const drkv_rope* r, int n_tokens, const int32_t* d_pos, cons
     p.rot_items = p.half / vw;
     p.row_items = p.rot_items + (copies ? (d - rot) / vw : 0);   // head_dim is a multiple of 8, rotary_dim of 2 vw
     p.magic_row = magic_of(p.row_items);
-    p.magic_heads = magic_of(p.heads);
     // Several tokens share a CTA once one each would be more than two waves of CTAs (8 of 256 threads an SM).
     p.tokens_per_cta = 1;
     while (p.tokens_per_cta < 8 && (int64_t)n_tokens > (int64_t)r->num_sms * 16 * p.tokens_per_cta) p.tokens_per_cta *= 2;
     while (p.tokens_per_cta > 1 && (int64_t)p.tokens_per_cta * p.heads * p.row_items > (1 << 16)) p.tokens_per_cta /= 2;
-    const int grid = (n_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
-    const size_t smem = (size_t)p.tokens_per_cta * 2 * ((p.half + 3) & ~3) * sizeof(float);
+    // the row kernel takes heads of 64, 128 and 256 dims (their lanes divide a warp) in 16-byte vectors
+    const bool by_rows = wide_rows && (d == 64 || d == 128 || d == 256);
+    const int mode = p.pairs_layout ? kPairs : rot % 16 == 0 ? kHalves : kAnyHalves;
+    const int ctas = (n_tokens + p.tokens_per_cta - 1) / p.tokens_per_cta;
+    // Few tokens: the heads are spread over CTAs too, as many as go at once in each (one token of 72 heads of 128: 1.8 us, in one CTA 3.3).
+    const int at_once = by_rows ? kRopeThreads / (d / 8) : p.row_items < kRopeThreads ? kRopeThreads / p.row_items : 1;
+    int parts = (p.heads + at_once - 1) / at_once;
+    if (parts > 2 * r->num_sms / ctas) parts = 2 * r->num_sms / ctas > 0 ? 2 * r->num_sms / ctas : 1;
+    p.heads_per_cta = (p.heads + parts - 1) / parts;
+    p.magic_heads = magic_of(p.heads_per_cta);
+    const dim3 grid(ctas, (p.heads + p.heads_per_cta - 1) / p.heads_per_cta);
+    const int pad = by_rows && mode == kAnyHalves ? (rot + 7) & ~7 : (p.half + 3) & ~3;
+    size_t smem = (size_t)p.tokens_per_cta * 2 * pad * sizeof(float);
     DeviceGuard dev(r->cfg.device);
     if (!dev.ok()) return fail(DRKV_ERR_CUDA, "rope_apply: cudaSetDevice failed");
-    // the row kernel takes heads of 64, 128 and 256 dims (their lanes divide a warp) in 16-byte vectors
-    if (wide_rows && (d == 64 || d == 128 || d == 256) && (r->cfg.layout == DRKV_ROPE_PAIRS || rot % 16 == 0)) {
+    if (by_rows) {
         const int lg = d == 64 ? 3 : d == 128 ? 4 : 5;
-        const bool pairs = r->cfg.layout == DRKV_ROPE_PAIRS, f16 = r->cfg.dtype == DRKV_DTYPE_F16;
+        if (mode == kAnyHalves) smem += (size_t)(kRopeThreads >> lg) * ring_elements(1 << lg) * 2;
         const cudaStream_t st = (cudaStream_t)stream;
-        const cudaError_t e = f16 ? (pairs ? launch_pdl(rope_rows_kernel<__half, true>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg)
-                                           : launch_pdl(rope_rows_kernel<__half, false>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg))
-                                  : (pairs ? launch_pdl(rope_rows_kernel<__nv_bfloat16, true>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg)
-                                           : launch_pdl(rope_rows_kernel<__nv_bfloat16, false>, dim3(grid), dim3(kRopeThreads), smem, st, p, lg));
+        const cudaError_t e = r->cfg.dtype == DRKV_DTYPE_F16 ? launch_rows<__half>(p, mode, lg, grid, smem, st)
+                                                             : launch_rows<__nv_bfloat16>(p, mode, lg, grid, smem, st);
         if (e != cudaSuccess) return fail(DRKV_ERR_CUDA, cudaGetErrorString(e));
         return DRKV_OK;
     }

@@ -136,6 +136,33 @@ def test_against_formula(drkv_lib, dtype, layout, d, rot, tokens, inverse):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("d,rot,hq,hkv,tokens", [(128, 128, 64, 8, 1), (128, 34, 60, 5, 5), (64, 62, 33, 0, 2), (256, 142, 19, 4, 40),
+                                                 (128, 116, 31, 1, 2500), (64, 2, 3, 3, 700), (96, 90, 50, 7, 3)])
+def test_many_heads_few_tokens_odd_halves(drkv_lib, layout, d, rot, hq, hkv, tokens):
+    """Heads spread over several CTAs (the last with fewer), halves that begin inside a 16-byte vector; out of place and in place."""
+    import torch
+    from deusridet_b200 import Rope
+    g = torch.Generator(device="cuda").manual_seed(d + rot + tokens)
+    rope = Rope(head_dim=d, rotary_dim=rot, theta=1e4, layout=layout, dtype="f16", device=0)
+    freq, a = expected_frequencies(rot, 1e4, "none")
+    q = torch.randn(tokens, hq, d, generator=g, device="cuda").half()
+    k = torch.randn(tokens, hkv, d, generator=g, device="cuda").half() if hkv else None
+    pos = torch.randint(0, 2 ** 20, (tokens,), generator=g, device="cuda", dtype=torch.int32)
+    q_out, k_out = rope.apply(pos, q, k)
+    _check(q_out, q, pos, freq, a, layout, False, torch.float16)
+    assert torch.equal(q_out[..., rot:], q[..., rot:])
+    if hkv:
+        _check(k_out, k, pos, freq, a, layout, False, torch.float16)
+    keep = torch.nan * torch.ones(tokens, hq + 1, d, device="cuda", dtype=torch.float16)      # a head behind, left as it was
+    keep[:, :hq] = q
+    rope.apply(pos, keep[:, :hq], k, out_q=keep[:, :hq], out_k=k)
+    torch.cuda.synchronize()
+    assert torch.equal(keep[:, :hq], q_out) and torch.isnan(keep[:, hq]).all()
+    assert k is None or torch.equal(k, k_out)
+
+
+@pytest.mark.gpu
 def test_strides_orders_alignment(drkv_lib):
     """Head-major storage, rows starting at odd elements, one tensor only, k alone, no tokens."""
     import torch
