@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kThreads8 = 256;
 constexpr int kMaxTokens8 = 32;   // tokens of one CTA of the append
+constexpr int kExpandCtas = 592;    // two waves of two an SM
 constexpr int kBatch8 = 4;        // rows a lane has in flight
 
 // Quantises the row of which each of its LANES lanes holds 8 elements; row: its index in the block's rows (K plane, then V
@@ -249,9 +250,11 @@ __device__ __forceinline__ Vec16 finite8(Vec16 v) {
     return v;
 }
 
-// grid (logical pages, sequences).  Of several sequences that share a page the one that sees the most tokens (the later
-// one of equals) writes it.  Slots past its last token may hold anything an earlier owner of the page left, and the attention
-// multiplies hidden values by zero: what is not finite there is written as zero.
+// grid (logical pages, sequences, parts of a page).  Slots past a sequence's last token may hold anything an earlier owner of
+// the page left, and the attention multiplies hidden values by zero: what is not finite there is written as zero.  So of
+// several places in tables that name one page the one that sees the most of it has to be the last word: a sequence's last
+// page is left to any place that sees more, and of sequences that share the place in their tables the longest writes (the
+// later one of equals; this only saves work).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params p) {
     constexpr int LANES = D / 8;
@@ -262,18 +265,27 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
     if ((int64_t)logical * P >= n_tok || logical >= p.table_stride) return;
     const int page = __ldg(p.tables + (int64_t)p.row[s] * p.table_stride + logical);
     if (page < 0 || page >= p.layout.max_pages) return;
+    const int visible = min(P, n_tok - logical * P);
+    if (visible < P) {
+        int seen = 0;
+        for (int o = 0; o < p.n_seq; o++) {
+            const int32_t* table = p.tables + (int64_t)p.row[o] * p.table_stride;
+            for (int l = threadIdx.x; l < p.table_stride && (int64_t)l * P < p.n_tokens[o]; l += kThreads8)
+                seen |= p.n_tokens[o] - l * P > visible && __ldg(table + l) == page;
+        }
+        if (__syncthreads_or(seen)) return;
+    }
     for (int o = 0; o < p.n_seq; o++) {
         if (o == s || (int64_t)logical * P >= p.n_tokens[o]) continue;
         if (p.n_tokens[o] < n_tok || (p.n_tokens[o] == n_tok && o < s)) continue;
         if (__ldg(p.tables + (int64_t)p.row[o] * p.table_stride + logical) == page) return;
     }
-    const int visible = min(P, n_tok - logical * P);
     const int rows = 2 * p.layout.num_kv_heads * P;                  // K rows then V rows, exponents in the same order
     const uint8_t* block = p.pool + p.layout.block_of(p.layer, page);
     const uint8_t* exps = block + 2 * p.layout.plane;
     T* image = reinterpret_cast<T*>(p.image) + (int64_t)page * rows * D;
     const int total = rows * LANES;
-    for (int i0 = threadIdx.x; i0 < total; i0 += kBatch8 * kThreads8) {
+    for (int i0 = threadIdx.x + blockIdx.z * kBatch8 * kThreads8; i0 < total; i0 += gridDim.z * kBatch8 * kThreads8) {
         uint2 q[kBatch8];
         uint8_t e[kBatch8];
 #pragma unroll
@@ -345,7 +357,11 @@ struct InjectLaunch {
 template <typename T, int D>
 struct ExpandLaunch {
     static cudaError_t run(const Expand8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(expand8_kernel<T, D>, dim3(n, p.n_seq), dim3(kThreads8), 0, s, p);
+        // Parts of one batch while the pages are few (one page of 128 tokens of 5 heads of 256: a 43-token chunk takes
+        // 51 us in one part, 13 in forty).
+        const int batches = (2 * p.layout.num_kv_heads * p.layout.page_size * (D / 8) + kBatch8 * kThreads8 - 1) / (kBatch8 * kThreads8);
+        const int parts = min(batches, max(1, kExpandCtas / (n * p.n_seq)));
+        return launch_pdl(expand8_kernel<T, D>, dim3(n, p.n_seq, parts), dim3(kThreads8), 0, s, p);
     }
 };
 

@@ -416,6 +416,34 @@ def test_prefill_over_the_pool(drkv_lib, dtype, d, grp, page):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("page,hkv,d,n,m", [(128, 5, 256, 43, 43), (128, 8, 64, 130, 2), (64, 3, 128, 1, 1)])
+def test_prefill_of_few_large_pages(drkv_lib, page, hkv, d, n, m):
+    """Pages that several CTAs expand, the last one only in part visible."""
+    import torch
+    eng = _engine(hq=hkv, hkv=hkv, d=d, page=page, dtype="bf16", pages=4, seqs=2, per_seq=2)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, n)
+    eng.set_seq_len(0, n)
+    eng.pool_tensor().fill_(-1)
+    eng.sync_block_table()
+    stored = _fill(eng, [n], "bf16", 3, spread=1)[0]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q = torch.randn(m, hkv, d, generator=g, device="cuda").bfloat16()
+    out = torch.zeros_like(q)
+    scale = 1.0 / math.sqrt(d)
+    eng.attend_prefill_batch(0, [0], [n - m], [m], [q], [out], scale)
+    torch.cuda.synchronize()
+    eng.check_kernels()
+    for t in range(m):
+        end = n - m + t + 1
+        for h in range(hkv):
+            want, pv, mag = R.attend(q[t, h:h + 1].double().cpu().numpy(), stored[0][:end, h], stored[1][:end, h], scale)
+            tol = R.attend_tolerance(want, pv, mag, _half_step("bf16"), _half_step("bf16"))
+            assert (np.abs(out[t, h:h + 1].double().cpu().numpy() - want) <= tol).all(), (t, h)
+    eng.close()
+
+
+@pytest.mark.gpu
 def test_prefill_pages_shared_out_of_step(drkv_lib):
     """One page at different places of two sequences' tables, whole for one and the tail of the other, in one call."""
     import torch
@@ -441,6 +469,20 @@ def test_prefill_pages_shared_out_of_step(drkv_lib):
             want, pv, mag = R.attend(qs[i][t].double().cpu().numpy(), stored[0][see, 0], stored[1][see, 0], 0.125)
             tol = R.attend_tolerance(want, pv, mag, _half_step("bf16"), _half_step("bf16"))
             assert (np.abs(outs[i][t].double().cpu().numpy() - want) <= tol).all(), (i, t)
+    # a NaN in a slot that the parent sees and the other's last page hides: the parent's answer is that of a call of its own
+    block = eng.pool_tensor().reshape(8, -1)[pages[0]]
+    for plane in (0, 1):
+        block[(plane * 16 + 9) * 32:(plane * 16 + 10) * 32] = -1
+    alone = torch.zeros_like(outs[0])
+    eng.attend_prefill_chunk(0, 0, 44, 4, qs[0], alone, 0.125)
+    assert not torch.equal(alone, outs[0])
+    for first, second in ((0, other), (other, 0)):
+        again = {0: torch.zeros_like(outs[0]), other: torch.zeros_like(outs[1])}
+        slot = {0: 0, other: 1}
+        eng.attend_prefill_batch(0, [first, second], [(44, 16)[slot[x]] for x in (first, second)], [4, 4],
+                                 [qs[slot[x]] for x in (first, second)], [again[first], again[second]], 0.125)
+        torch.cuda.synchronize()
+        assert torch.equal(again[0].view(torch.int16), alone.view(torch.int16))
     eng.close()
 
 
