@@ -11,8 +11,8 @@
 // small kernel merges them in a fixed order (results do not depend on timing).  Warps of one CTA take stretches far apart,
 // so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and then by the last CTA to arrive, took
 // 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end.
-// Bound by HBM: the loop over groups reads 7 TB/s (131 001 keys of 8 heads, 270 MB: 50 us, 8 more for the merge; 64 sequences
-// of 1-8 k keys, 602 MB: 106 us); what is left is the first data of a launch, the uneven finish and the merge.
+// Bound by HBM: the loop over groups reads 7 TB/s (131 001 keys of 8 heads, 270 MB: 50 us, 5 more for the merge; 64 sequences
+// of 1-8 k keys, 602 MB: 106 us and 4); what is left is the first data of a launch, the uneven finish and the merge.
 //
 // A warp brings its groups into a private ring of shared memory by cp.async (16 bytes a lane, L1 bypassed), kStages - 1
 // groups ahead, and reads them as matrix operands without ldmatrix: contraction order is free, so a lane takes whole
