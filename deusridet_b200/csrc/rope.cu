@@ -13,6 +13,7 @@
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "device_guard.hpp"
@@ -56,7 +57,9 @@ struct RopeParams {
 };
 
 // Cosines and sines of a CTA's tokens, one pair per thread: [token][cosines | sines][pad].  PER_DIM: one of each for every
-// dim that turns, the sine with the sign that the dim's own formula gives it.
+// dim that turns, the sine with the sign that the dim's own formula gives it; a lane's eight as two vectors that stand where
+// its neighbours' do not collide (trig_place).
+__device__ __forceinline__ int trig_place(int dim, int pad) { return (dim & 4 ? pad / 2 : 0) + (dim >> 3) * 4 + (dim & 3); }
 template <bool PER_DIM>
 __device__ __forceinline__ void fill_trig(const RopeParams& p, float* s_trig, int tok0, int n_tok, int pad) {
     const int n = PER_DIM ? p.half : pad;
@@ -69,12 +72,14 @@ __device__ __forceinline__ void fill_trig(const RopeParams& p, float* s_trig, in
             sincospif((float)hi * 0x1p-31f, &s, &c);
             c *= p.factor;
             s = (p.inverse ? -s : s) * p.factor;
-            float* to = s_trig + t * 2 * pad + j;
-            to[0] = c;
-            to[pad] = PER_DIM ? -s : s;
+            float* to = s_trig + t * 2 * pad;
+            const int at = PER_DIM ? trig_place(j, pad) : j;
+            to[at] = c;
+            to[pad + at] = PER_DIM ? -s : s;
             if (PER_DIM) {
-                to[p.half] = c;
-                to[pad + p.half] = s;
+                const int beside = trig_place(j + p.half, pad);
+                to[beside] = c;
+                to[pad + beside] = s;
             }
         }
     }
@@ -175,14 +180,16 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 // (The general kernel above loses on them by index arithmetic per vector: 158 us.)
 // Halves of a width that is no multiple of 8 (kAnyHalves): a lane's partners lie across two vectors, so a warp lays the row
 // into shared memory as a ring (the first half once more behind the second), where the partner of dim e is at e + half
-// (50 of 64 dims of 28 heads, 7 401 tokens: 20 us; the general kernel, by single elements, 36).
+// (50 of 64 dims of 28 heads, 7 401 tokens: 17 us; the general kernel, by single elements, 39.  116 of 128 dims of 36 heads,
+// 16 824 tokens: 84 us; by words 104; this with the row read back by words and a lane's cosines side by side 110: shared
+// memory's banks are what it is short of).
 enum RopeMode { kHalves, kPairs, kAnyHalves };
 
 // Elements of a row's ring: rotary_dim + half, and what a lane reads past its own.
 __host__ __device__ constexpr int ring_elements(int lanes) { return 12 * lanes + 16; }
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 5 : 8) rope_rows_kernel(const RopeParams p, int lanes_log2) {
+__global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 4 : 8) rope_rows_kernel(const RopeParams p, int lanes_log2) {
     constexpr bool PAIRS = MODE == kPairs, ANY = MODE == kAnyHalves;
     extern __shared__ __align__(16) float s_trig[];             // [tokens_per_cta][2][pad], then the rows' rings
     pdl_wait();
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 5 : 8) rope
     const int live_pairs = half - 4 * l;                        // of the lane's four words, those that turn (not kHalves)
     const bool second = !PAIRS && l >= half_lanes;
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
-    const int trig0 = !turns ? 0 : PAIRS ? 4 * l : ANY ? 8 * l : 8 * (second ? l - half_lanes : l);
+    const int trig0 = !turns ? 0 : PAIRS || ANY ? 4 * l : 8 * (second ? l - half_lanes : l);
     const int ring = ring_elements(lanes);
     uint32_t* row_ring = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(s_trig + p.tokens_per_cta * 2 * pad) + (threadIdx.x >> lanes_log2) * ring);
     struct Row {
@@ -222,22 +229,39 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 5 : 8) rope
         float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < (PAIRS ? 1 : 2); i++) {
-            *reinterpret_cast<float4*>(c + 4 * i) = cs[i];
-            *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + i];
+            *reinterpret_cast<float4*>(c + 4 * i) = cs[ANY ? pad / 8 * i : i];
+            *reinterpret_cast<float4*>(s + 4 * i) = cs[pad / 4 + (ANY ? pad / 8 * i : i)];
         }
         Vec16 y, other = x.v;
         if (ANY) {
             __syncwarp();                                       // the row before has been read
+            if (live_pairs >= 4) *reinterpret_cast<Vec16*>(row_ring + 4 * l) = x.v;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (i < live_pairs) row_ring[4 * l + i] = x.v.w[i];
+                if (live_pairs < 4 && i < live_pairs) row_ring[4 * l + i] = x.v.w[i];
                 if (8 * l + 2 * i < half) row_ring[half + 4 * l + i] = x.v.w[i];
             }
             __syncwarp();
             if (turns) {
-                const uint32_t* from = row_ring + ((8 * l + half) >> 1);
+                // the two vectors that hold dims 8 l + half and on, shifted to their first
+                const Vec16* from = reinterpret_cast<const Vec16*>(row_ring) + ((8 * l + half) >> 3);
+                const Vec16 v0 = from[0], v1 = from[1];
+                const uint32_t bits = half & 1 ? 16 : 0;
+                auto shifted = [&](auto words) {
+                    constexpr int W = decltype(words)::value;
 #pragma unroll
-                for (int i = 0; i < 4; i++) other.w[i] = __funnelshift_r(from[i], from[i + 1], half & 1 ? 16 : 0);
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t lo = i + W < 4 ? v0.w[(i + W) & 3] : v1.w[(i + W) & 3];
+                        const uint32_t hi = i + W + 1 < 4 ? v0.w[(i + W + 1) & 3] : v1.w[(i + W + 1) & 3];
+                        other.w[i] = __funnelshift_r(lo, hi, bits);
+                    }
+                };
+                switch (half >> 1 & 3) {
+                    case 0: shifted(std::integral_constant<int, 0>{}); break;
+                    case 1: shifted(std::integral_constant<int, 1>{}); break;
+                    case 2: shifted(std::integral_constant<int, 2>{}); break;
+                    default: shifted(std::integral_constant<int, 3>{}); break;
+                }
             }
         }
 #pragma unroll
