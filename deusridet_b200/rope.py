@@ -64,10 +64,19 @@ class Rope:
                              f"{tuple(to_shape)} {dst.dtype} {dst.device}")
         return RopeRows(src.data_ptr(), dst.data_ptr(), shape[1], strides[0], strides[1], to_strides[0], to_strides[1])
 
+    def _new(self, like, stream):
+        import torch
+        if stream is None:
+            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        # the allocator may hand out memory that earlier work of the stream it believes to be current still uses
+        with torch.cuda.stream(torch.cuda.ExternalStream(_stream(stream), device=self.device)):
+            return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+
     def apply(self, pos, q=None, k=None, *, out_q=None, out_k=None, inverse: bool = False, stream=None):
         """Rotates q and k, tensors [n_tokens, heads, head_dim] of any token and head strides, by the int32 positions
         `pos` [n_tokens]; into out_q / out_k (new contiguous tensors by default; the input itself for in place).
-        inverse=True applies the transpose, the gradient.  Returns (out_q, out_k)."""
+        inverse=True applies the transpose, the gradient.  Runs on `stream`, by default the device's current one; new outputs
+        belong to it.  Returns (out_q, out_k)."""
         import torch
         if q is None and k is None:
             raise ValueError("nothing to rotate: give q, k or both")
@@ -80,11 +89,12 @@ class Rope:
         q_rows = k_rows = None
         if q is not None:
             if out_q is None:
-                out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                out_q = self._new(q, stream)
             q_rows = C.byref(self._rows(q, out_q, n, "q"))
         if k is not None:
             if out_k is None:
-                out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+                out_k = self._new(k, stream)
             k_rows = C.byref(self._rows(k, out_k, n, "k"))
-        check(self.lib.drkv_rope_apply(self.h, n, pos.data_ptr(), q_rows, k_rows, 1 if inverse else 0, _stream(stream)))
+        check(self.lib.drkv_rope_apply(self.h, n, pos.data_ptr(), q_rows, k_rows, 1 if inverse else 0,
+                                       _stream(torch.cuda.current_stream(self.device) if stream is None else stream)))
         return out_q, out_k

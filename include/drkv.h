@@ -516,7 +516,8 @@ typedef struct drkv_rope_config {
     double theta, factor;
 } drkv_rope_config;
 /* Rows of one tensor, strides in elements: element (token, head, dim) is at token * token_stride + head * head_stride +
- * dim.  src may be dst with the same strides (in place); other overlaps are refused. */
+ * dim.  src may be dst with the same strides (in place); other overlaps of the two are refused.  What one tensor writes may
+ * not be an element of the other's rows (they may lie between one another, as in a fused projection). */
 typedef struct drkv_rope_rows {
     const void* src;
     void* dst;

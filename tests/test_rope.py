@@ -190,6 +190,37 @@ def test_strides_orders_alignment(drkv_lib):
 
 
 @pytest.mark.gpu
+def test_streams(drkv_lib):
+    """The current stream by default (a capture too), a given one as an object or a handle, with outputs allocated for it."""
+    import torch
+    from deusridet_b200 import Rope
+    rope = Rope(head_dim=128, dtype="bf16", device=0)
+    pos = torch.arange(4000, device="cuda", dtype=torch.int32)
+    q = torch.randn(4000, 8, 128, device="cuda").bfloat16()
+    want, _ = rope.apply(pos, q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            x = q + 0
+            got, _ = rope.apply(pos, x, out_q=x)                     # in place right behind the copy, on its stream
+    side.synchronize()
+    assert torch.equal(got, want)
+    for stream in (side, side.cuda_stream, torch.cuda.default_stream().cuda_stream):
+        torch.cuda.synchronize()
+        got, _ = rope.apply(pos, q, stream=stream)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, _ = rope.apply(pos, q)
+    got.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_argument_checks_on_tensors(drkv_lib):
     import torch
     from deusridet_b200 import DrkvError, Rope
