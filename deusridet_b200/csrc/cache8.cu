@@ -17,24 +17,25 @@ namespace drkv {
 namespace {
 
 constexpr int kThreads8 = 256;
-constexpr int kMaxTokens8 = 32;   // tokens of one CTA of the append
+constexpr int kMaxTokens8 = 128;  // tokens of one CTA of the append
 constexpr int kExpandCtas = 592;    // two waves of two an SM
 constexpr int kBatch8 = 4;        // rows a lane has in flight
 
-// Quantises the row of which each of its LANES lanes holds 8 elements; row: its index in the block's rows (K plane, then V
-// plane, exponents in the same order).
-template <int LANES>
-__device__ __forceinline__ void quantise_row(const float (&x)[8], uint8_t* block, int64_t exponents, int row, int l, bool store) {
+// Quantises the row of which each of its LANES lanes holds NV runs of 8 elements, runs l, l + LANES ...; row: its index in the
+// block's rows (K plane, then V plane, exponents in the same order).
+template <int LANES, int NV>
+__device__ __forceinline__ void quantise_row(const float (&x)[8 * NV], uint8_t* block, int64_t exponents, int row, int l, bool store) {
     // the maximum of |x|; NaN is passed over by the maximum, an infinity makes the row look again
-    float top = fmax3(fmaxf(fabsf(x[0]), fabsf(x[1])), fabsf(x[2]), fabsf(x[3]));
-    top = fmax3(fmax3(top, fabsf(x[4]), fabsf(x[5])), fabsf(x[6]), fabsf(x[7]));
+    float top = fmaxf(fabsf(x[0]), fabsf(x[1]));
+#pragma unroll
+    for (int i = 2; i < 8 * NV; i += 2) top = fmax3(top, fabsf(x[i]), fabsf(x[i + 1]));
     uint32_t amax = __float_as_uint(top == top ? top : 0.f);
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (__any_sync(0xffffffffu, amax >= 0x7f800000u)) {
         amax = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
+        for (int i = 0; i < 8 * NV; i++) {
             const uint32_t a = __float_as_uint(x[i]) & 0x7fffffffu;
             amax = max(amax, a < 0x7f800000u ? a : 0u);
         }
@@ -43,17 +44,21 @@ __device__ __forceinline__ void quantise_row(const float (&x)[8], uint8_t* block
     }
     const int e = e4m3_row_exponent(amax);
     const float inv = exp2_int(-e);
-    uint2 v;
-    v.x = f32x4_to_e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-    v.y = f32x4_to_e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-    if (store) {
-        *reinterpret_cast<uint2*>(block + (int64_t)row * (8 * LANES) + 8 * l) = v;
-        if (l == 0) block[exponents + row] = (uint8_t)(e + 127);
+    if (!store) return;
+    uint8_t* to = block + (int64_t)row * (8 * LANES * NV) + 8 * l;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const float* y = x + 8 * v;
+        uint2 q;
+        q.x = f32x4_to_e4m3x4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+        q.y = f32x4_to_e4m3x4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
+        *reinterpret_cast<uint2*>(to + 8 * LANES * v) = q;
     }
+    if (l == 0) block[exponents + row] = (uint8_t)(e + 127);
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack8(const Vec16& v, float (&x)[8]) {
+__device__ __forceinline__ void unpack8(const Vec16& v, float* x) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 f = Elem<T>::unpack2(v.w[i]);
@@ -101,11 +106,14 @@ struct TokenPlace {
     int slot, pos;
 };
 
-// A CTA takes some tokens, D / 8 lanes per row: a token's K heads, then its V heads, as in its page block.  The next row is
-// on its way while one is worked on (30 001 tokens of 4 heads of 256: 41 us, 4.5 TB/s; one token a CTA and no read ahead: 77).
+// A CTA takes some tokens, D / 16 lanes per row, two runs of 8 elements a lane: a token's K heads, then its V heads, as in its
+// page block.  The next row is on its way while one is worked on.  Bound by instructions: 30 001 tokens of 4 heads of 256 take
+// APPUS us; one run a lane 41, and without the read ahead, a token a CTA, 77.
+constexpr int kAppendRuns = 2;
+struct RowRuns { Vec16 v[kAppendRuns]; };
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads8, 6) append8_kernel(const Append8Params p, int n_all, int tokens_per_cta, uint32_t magic_rows) {
-    constexpr int LANES = D / 8, ROWS = kThreads8 / LANES;
+__global__ void __launch_bounds__(kThreads8, 4) append8_kernel(const Append8Params p, int n_all, int tokens_per_cta, uint32_t magic_rows) {
+    constexpr int NV = kAppendRuns, LANES = D / (8 * NV), ROWS = kThreads8 / LANES;
     extern __shared__ float s_trig[];                                // [token][2][half]
     __shared__ TokenPlace s_place[kMaxTokens8];
     pdl_wait();
@@ -114,14 +122,17 @@ __global__ void __launch_bounds__(kThreads8, 6) append8_kernel(const Append8Para
     const int P = p.layout.page_size, H = p.layout.num_kv_heads;
     const int l = threadIdx.x % LANES, total = n_tok * 2 * H;
     const int64_t exponents = 2 * p.layout.plane;
-    auto read = [&](int r) -> Vec16 {
-        if (r >= total) return Vec16{{0u, 0u, 0u, 0u}};
+    auto read = [&](int r) -> RowRuns {
+        RowRuns x{};
+        if (r >= total) return x;
         const int t = div_magic(r, magic_rows), kh = r - t * 2 * H;
         const T* src = reinterpret_cast<const T*>(kh < H ? p.k_src : p.v_src) + ((int64_t)(tok0 + t) * H + (kh < H ? kh : kh - H)) * D;
-        return ldg16(src + 8 * l);
+#pragma unroll
+        for (int v = 0; v < NV; v++) x.v[v] = ldg16(src + 8 * (l + v * LANES));
+        return x;
     };
     const int r_own = threadIdx.x / LANES;
-    Vec16 a = read(r_own), b;                                        // on its way while the places are worked out
+    RowRuns a = read(r_own), b;                                      // on its way while the places are worked out
     if (threadIdx.x < n_tok) {
         const int tok = tok0 + threadIdx.x;
         int row = p.row, pos = p.pos_start + tok;
@@ -145,28 +156,45 @@ __global__ void __launch_bounds__(kThreads8, 6) append8_kernel(const Append8Para
         }
         __syncthreads();
     }
-    auto write = [&](const Vec16& in, int r) {
+    auto write = [&](const RowRuns& in, int r) {
         const int t = div_magic(min(r, total - 1), magic_rows), kh = min(r, total - 1) - t * 2 * H;
-        float x[8];
-        unpack8<T>(in, x);
-        if (half > 0) {
-            const int hl = half / 8;                                 // lanes of one rotated half (rotary_dim % 16 == 0)
-            const bool first = l < hl, second = l >= hl && l < 2 * hl;
-            // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
-            const int base = (threadIdx.x & 31) - l, other = base + (first ? l + hl : second ? l - hl : l);
-            const float* c = s_trig + 2 * t * half + 8 * (first ? l : second ? l - hl : 0);
+        float x[8 * NV];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float o = __shfl_sync(0xffffffffu, x[i], other);
+        for (int v = 0; v < NV; v++) unpack8<T>(in.v[v], x + 8 * v);
+        if (half > 0 && __any_sync(0xffffffffu, kh < H)) {
+            const int hl = half / 8;                                 // runs of one rotated half (rotary_dim % 16 == 0)
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                const int run = l + v * LANES;
+                const bool first = run < hl, second = run >= hl && run < 2 * hl;
+                const int other = first ? run + hl : second ? run - hl : run;
+                // a shuffle within the row's lanes: LANES divides 32 and rows are aligned groups of lanes
+                const int from = (threadIdx.x & 31) - l + other % LANES;
+                float o[8];
+                Vec16 partner;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    partner.w[i] = __shfl_sync(0xffffffffu, in.v[0].w[i], from);
+#pragma unroll
+                    for (int u = 1; u < NV; u++) {
+                        const uint32_t w = __shfl_sync(0xffffffffu, in.v[u].w[i], from);
+                        if (other / LANES == u) partner.w[i] = w;
+                    }
+                }
+                unpack8<T>(partner, o);
                 if (kh < H && (first || second)) {
-                    float y0, y1;
-                    rope_pair(first ? x[i] : o, first ? o : x[i], c[i], c[half + i], y0, y1);
-                    x[i] = first ? y0 : y1;
+                    const float* c = s_trig + 2 * t * half + 8 * (first ? run : run - hl);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float y0, y1, &mine = x[8 * v + i];
+                        rope_pair(first ? mine : o[i], first ? o[i] : mine, c[i], c[half + i], y0, y1);
+                        mine = first ? y0 : y1;
+                    }
                 }
             }
         }
         const TokenPlace at = s_place[t];
-        quantise_row<LANES>(x, p.pool + at.block, exponents, kh * P + at.slot, l, r < total && at.block >= 0);
+        quantise_row<LANES, NV>(x, p.pool + at.block, exponents, kh * P + at.slot, l, r < total && at.block >= 0);
     };
     for (int r0 = 0; r0 < total; r0 += 2 * ROWS) {                   // the whole CTA together: rows r0 + r_own, then the next
         b = read(r0 + ROWS + r_own);
@@ -232,7 +260,7 @@ __global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params
                 const TokenPlace at = s_place[t];
                 float x[8];
                 unpack8<T>(in[u], x);
-                quantise_row<LANES>(x, p.pool + at.block, exponents, (kv * H + h) * P + at.slot, l, r < total && at.block >= 0);
+                quantise_row<LANES, 1>(x, p.pool + at.block, exponents, (kv * H + h) * P + at.slot, l, r < total && at.block >= 0);
             }
         }
     }
@@ -332,14 +360,17 @@ cudaError_t by_shape(const P& p, int dtype, int head_dim, int n, cudaStream_t st
 template <typename T, int D>
 struct AppendLaunch {
     static cudaError_t run(const Append8Params& p, int n, cudaStream_t s) {
-        // a token a CTA for decode batches; more, a dozen rows a lane and at most 32 tokens, while such CTAs fill the SMs twice
-        // over (6 of 256 threads each)
-        constexpr int ROWS = kThreads8 / (D / 8);
-        const int H = p.layout.num_kv_heads;
+        // A token a CTA for decode batches.  Tokens join while one wave of CTAs is left (4 of 256 threads an SM) until a lane
+        // has two rows, the first to work on while the other comes, then up to six while there are two waves; their angles have
+        // to fit 32 KB.  (4 097 tokens of 8 heads of 128, written and read: 11.5 us with two rows a lane, 13.0 with one.)
+        constexpr int ROWS = kThreads8 / (D / (8 * kAppendRuns));
+        const int rows = 2 * p.layout.num_kv_heads, wave = 4 * 148;
         int per = 1;
-        while (per < kMaxTokens8 && per * 2 * H < 12 * ROWS && n >= 2 * per * 2 * 6 * 148) per *= 2;
+        while (per < kMaxTokens8 && 2 * per * p.rotary_dim <= 8192 &&
+               ((per * rows < 2 * ROWS && n >= per * wave) || (per * rows < 6 * ROWS && n >= 2 * per * wave)))
+            per *= 2;
         return launch_pdl(append8_kernel<T, D>, dim3((n + per - 1) / per), dim3(kThreads8), (size_t)per * p.rotary_dim * sizeof(float),
-                          s, p, n, per, magic_of(2 * H));
+                          s, p, n, per, magic_of(rows));
     }
 };
 template <typename T, int D>

@@ -285,9 +285,10 @@ DRKV_API int drkv_append_attend_decode_planned(drkv_engine* e, int layer, const 
  * Bounds of a (layer, page, KV head), int8: b_max[d] = ceil(max k[d] / 2^e), b_min[d] = floor(min k[d] / 2^e) over the keys of
  * the page, e the smallest integer with max|k| <= 127 * 2^e (held within -126..121); NaN keys are ignored.
  * From drkv_page_bounds_enable on, every call of this engine that writes keys keeps them: a page starts anew when its slot
- * 0 is written and is widened by every other write, copies on write take them along, pages from the storage tier are
- * scanned.  The call itself scans every slot of every page (calling it again does so again: for a host that has written
- * through drkv_pool_ptr).  Bounds may be wider than a page's keys, never narrower.  Costs 1 / page_size of a 16-bit pool. */
+ * 0 is written (what it held is taken as gone) and is widened by every other write, copies on write take them along, pages
+ * from the storage tier are scanned.  The call itself scans every slot of every page (calling it again does so again: for a
+ * host that has written through drkv_pool_ptr, or has rewritten slot 0 of a page whose other slots it keeps).  Bounds may be
+ * wider than the keys written since then, never narrower.  Costs 1 / page_size of a 16-bit pool. */
 DRKV_API int drkv_page_bounds_enable(drkv_engine* e, void* stream);
 /* Device memory of the bounds, [layer][page][kv_head][b_max: head_dim, b_min: head_dim], and of their exponents,
  * [layer][page][kv_head]; NULL before drkv_page_bounds_enable. */
