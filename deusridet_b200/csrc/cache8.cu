@@ -108,7 +108,7 @@ struct TokenPlace {
 
 // A CTA takes some tokens, D / 16 lanes per row, two runs of 8 elements a lane: a token's K heads, then its V heads, as in its
 // page block.  The next row is on its way while one is worked on.  Bound by instructions: 30 001 tokens of 4 heads of 256 take
-// APPUS us; one run a lane 41, and without the read ahead, a token a CTA, 77.
+// 33 us, 5.6 TB/s; one run a lane 41, and without the read ahead, a token a CTA, 77.
 constexpr int kAppendRuns = 2;
 struct RowRuns { Vec16 v[kAppendRuns]; };
 template <typename T, int D>
@@ -205,17 +205,17 @@ __global__ void __launch_bounds__(kThreads8, 4) append8_kernel(const Append8Para
     }
 }
 
-// grid (token blocks, layer * 2 + plane): a CTA takes kFlatTokens tokens of one plane, four rows a lane at a time.
-constexpr int kFlatTokens = 16;
+// grid (token blocks, layer * 2 + plane): a CTA takes some tokens of one plane, four rows a lane at a time.
+constexpr int kFlatTokens = 64;   // at most
 template <typename T, int D, bool TO_FLAT>
-__global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params p, uint32_t magic_heads) {
+__global__ void __launch_bounds__(kThreads8) flat_copy8_kernel(const Flat8Params p, int tokens_per_cta, uint32_t magic_heads) {
     constexpr int LANES = D / 8, ROWS = kThreads8 / LANES;
     __shared__ TokenPlace s_place[kFlatTokens];
     pdl_wait();
     pdl_launch_dependents();
     const int H = p.layout.num_kv_heads, P = p.layout.page_size;
     const int layer = blockIdx.y >> 1, kv = blockIdx.y & 1;
-    const int tok0 = blockIdx.x * kFlatTokens, n_tok = min(kFlatTokens, p.num_tokens - tok0);
+    const int tok0 = blockIdx.x * tokens_per_cta, n_tok = min(tokens_per_cta, p.num_tokens - tok0);
     if (threadIdx.x < n_tok) {
         const int pos = p.start_token + tok0 + threadIdx.x, logical = pos / P;
         const int page = logical < p.table_stride ? __ldg(p.table + logical) : -1;
@@ -373,17 +373,25 @@ struct AppendLaunch {
                           s, p, n, per, magic_of(rows));
     }
 };
+// As many tokens a CTA as make one or two batches of rows a lane, fewer while the CTAs do not fill the SMs
+// (307 041 tokens of one head of 128 written and read: 83 us so, 110 with 16 a CTA; 1 592 tokens of 5 of 256: 7.8 and 8.4).
+template <typename T, int D, bool TO_FLAT>
+cudaError_t launch_flat8(const Flat8Params& p, cudaStream_t s) {
+    constexpr int ROWS = kThreads8 / (D / 8);
+    const int H = p.layout.num_kv_heads;
+    int per = kFlatTokens;
+    while (per > 1 && per * H >= 2 * kBatch8 * ROWS) per /= 2;
+    while (per > 1 && (int64_t)((p.num_tokens + per - 1) / per) * 2 * p.num_layers < 4 * 148) per /= 2;
+    return launch_pdl(flat_copy8_kernel<T, D, TO_FLAT>, dim3((p.num_tokens + per - 1) / per, 2 * p.num_layers), dim3(kThreads8), 0, s, p, per,
+                      magic_of(H));
+}
 template <typename T, int D>
 struct ExtractLaunch {
-    static cudaError_t run(const Flat8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(flat_copy8_kernel<T, D, true>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p, magic_of(p.layout.num_kv_heads));
-    }
+    static cudaError_t run(const Flat8Params& p, int, cudaStream_t s) { return launch_flat8<T, D, true>(p, s); }
 };
 template <typename T, int D>
 struct InjectLaunch {
-    static cudaError_t run(const Flat8Params& p, int n, cudaStream_t s) {
-        return launch_pdl(flat_copy8_kernel<T, D, false>, dim3(n, 2 * p.num_layers), dim3(kThreads8), 0, s, p, magic_of(p.layout.num_kv_heads));
-    }
+    static cudaError_t run(const Flat8Params& p, int, cudaStream_t s) { return launch_flat8<T, D, false>(p, s); }
 };
 template <typename T, int D>
 struct ExpandLaunch {
@@ -406,9 +414,8 @@ cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, cuda
 cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, cudaStream_t stream) {
     if (p.num_tokens <= 0) return cudaSuccess;
     if (p.num_layers > 32767) return cudaErrorInvalidValue;          // grid.y
-    const int blocks = (p.num_tokens + kFlatTokens - 1) / kFlatTokens;
-    return to_flat ? by_shape<ExtractLaunch>(p, dtype, p.layout.head_dim, blocks, stream)
-                   : by_shape<InjectLaunch>(p, dtype, p.layout.head_dim, blocks, stream);
+    return to_flat ? by_shape<ExtractLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, stream)
+                   : by_shape<InjectLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, stream);
 }
 
 cudaError_t launch_expand8(const Expand8Params& p, int dtype, cudaStream_t stream) {
