@@ -689,14 +689,16 @@ cudaError_t launch_one(const AttendPagesParams& p, int num_sms, cudaStream_t str
     const int n_warps = num_sms * R::kWarps;
     const int64_t pairs = (int64_t)p.n_seq * p.num_kv_heads, rows = pairs * p.group;
     // About n_warps / pairs pieces a row, eight of which a set of lanes takes at a time: the more pieces, the fewer dims a CTA
-    // takes and the more sets it has (60 rows of 118 pieces of 256 dims: 20 us a pass with four sets, 15 with thirty-two).
-    const int64_t pieces = n_warps / pairs + 2;
-    if (pieces > 8) {
+    // takes and the more sets it has (60 rows of 118 pieces of 256 dims: 20 us a pass with four sets, 15 with thirty-two), as
+    // long as the CTAs are resident in two turns (3 360 rows of 9 pieces of 64 dims, a CTA each: 43 us a pass; eight a CTA: 21).
+    const int64_t pieces = n_warps / pairs + 2, most = 4 * (int64_t)num_sms;
+    if (pieces > 8 && rows <= most) {
         constexpr int MID = D > 64 ? 64 : D;
-        if (pieces <= 8 * (1024 / D)) return launch_pdl(merge_pieces_kernel<T, D, D>, dim3((unsigned)rows), dim3(256), 0, stream, p, n_warps);
-        if (pieces <= 8 * (1024 / MID))
+        if (pieces > 8 * (1024 / MID) && rows * (D / 32) <= most)
+            return launch_pdl(merge_pieces_kernel<T, D, 32>, dim3((unsigned)rows, D / 32), dim3(256), 0, stream, p, n_warps);
+        if (pieces > 8 * (1024 / D) && rows * (D / MID) <= most)
             return launch_pdl(merge_pieces_kernel<T, D, MID>, dim3((unsigned)rows, D / MID), dim3(256), 0, stream, p, n_warps);
-        return launch_pdl(merge_pieces_kernel<T, D, 32>, dim3((unsigned)rows, D / 32), dim3(256), 0, stream, p, n_warps);
+        return launch_pdl(merge_pieces_kernel<T, D, D>, dim3((unsigned)rows), dim3(256), 0, stream, p, n_warps);
     }
     constexpr int per_cta = 128 / (D / 4);
     return launch_pdl(merge_pieces_kernel<T, D, 0>, dim3((unsigned)((rows + per_cta - 1) / per_cta)), dim3(128), 0, stream, p, n_warps);

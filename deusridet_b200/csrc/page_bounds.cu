@@ -56,26 +56,29 @@ __device__ __forceinline__ void load_key(const uint8_t* block, const BoundsParam
     }
 }
 
-// One warp per (page, KV head).  What a launch covers:
+// One warp per (page, KV head), or a CTA whose warps share the slots (SPLIT: what covers more than a token a page; 2 048
+// tokens of 8 heads of 256 on pages of 128: 9 us, by one warp each 63).  What a launch covers:
 //   rows != null    the page of every batch entry's position, that slot (entries of one sequence in the same page are
 //                   gathered by the first of them: one writer per page)
 //   table != null   the pages of one sequence that hold tokens [pos_start, pos_start + m), those slots
 //   neither         pages [page0, page0 + n_items), every slot
 // A page whose slot 0 is covered starts anew, any other is widened.
-template <bool POOL8, typename T, int D>
+template <bool POOL8, typename T, int D, bool SPLIT>
 __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
-    constexpr int C = D / 32;
+    constexpr int C = D / 32, WARPS = SPLIT ? 8 : 1;
+    __shared__ float s_hi[SPLIT ? 8 : 1][D], s_lo[SPLIT ? 8 : 1][D];
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t wid = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int w = threadIdx.x >> 5;
+    const int64_t wid = SPLIT ? blockIdx.x : (int64_t)blockIdx.x * 8 + w;
     const int item = (int)(wid / p.num_kv_heads), head = (int)(wid - (int64_t)item * p.num_kv_heads);
     if (item >= p.n_items) return;
     const int layer = p.layer + blockIdx.y;
     const int P = p.page_size;
     int page = -1, slot_lo = 0, slot_hi = P, row = 0, logical = 0;
     bool fresh = true;
-    if (p.rows != nullptr) {
+    if (!SPLIT && p.rows != nullptr) {
         row = __ldg(p.rows + item);
         const int pos = __ldg(p.pos + item) + p.pos_offset;
         if (pos < 0 || row < 0 || row >= p.max_rows) return;
@@ -124,8 +127,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
         }
     };
 #pragma unroll 4
-    for (int s = slot_lo; s < slot_hi; s++) take(s);
-    if (p.rows != nullptr) {                                                // later entries in the same page
+    for (int s = slot_lo + (SPLIT ? w : 0); s < slot_hi; s += WARPS) take(s);
+    if (!SPLIT && p.rows != nullptr) {                                                // later entries in the same page
         for (int j0 = item + 1; j0 < p.n_items; j0 += 32) {
             const int j = j0 + lane;
             int slot = -1;
@@ -139,6 +142,22 @@ __global__ void __launch_bounds__(256) bounds_kernel(const BoundsParams p) {
                 fresh |= s == 0;
             }
         }
+    }
+    if (SPLIT) {
+#pragma unroll
+        for (int i = 0; i < C; i++) {
+            s_hi[w][lane + 32 * i] = hi[i];                                 // channel lane * C + i
+            s_lo[w][lane + 32 * i] = lo[i];
+        }
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int v = 1; v < WARPS; v++)
+#pragma unroll
+            for (int i = 0; i < C; i++) {
+                hi[i] = fmaxf(hi[i], s_hi[v][lane + 32 * i]);
+                lo[i] = fminf(lo[i], s_lo[v][lane + 32 * i]);
+            }
     }
     if (!fresh) {
         const float unit = exp2_int(p.exponents[at]);
@@ -552,9 +571,12 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const Selec
 template <bool POOL8, typename T>
 cudaError_t launch_bounds_d(const BoundsParams& p, int head_dim, dim3 grid, cudaStream_t s) {
     switch (head_dim) {
-        case 64: return launch_pdl(bounds_kernel<POOL8, T, 64>, grid, dim3(256), 0, s, p);
-        case 128: return launch_pdl(bounds_kernel<POOL8, T, 128>, grid, dim3(256), 0, s, p);
-        case 256: return launch_pdl(bounds_kernel<POOL8, T, 256>, grid, dim3(256), 0, s, p);
+        case 64: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 64, true>, grid, dim3(256), 0, s, p)
+                                         : launch_pdl(bounds_kernel<POOL8, T, 64, false>, grid, dim3(256), 0, s, p);
+        case 128: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 128, true>, grid, dim3(256), 0, s, p)
+                                         : launch_pdl(bounds_kernel<POOL8, T, 128, false>, grid, dim3(256), 0, s, p);
+        case 256: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 256, true>, grid, dim3(256), 0, s, p)
+                                         : launch_pdl(bounds_kernel<POOL8, T, 256, false>, grid, dim3(256), 0, s, p);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -587,7 +609,8 @@ cudaError_t launch_score(const SelectParams& p, int num_sms, cudaStream_t s) {
 
 cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, cudaStream_t stream) {
     if (p.n_items <= 0 || num_layers <= 0) return cudaSuccess;
-    const int64_t blocks = ((int64_t)p.n_items * p.num_kv_heads + 7) / 8;
+    const bool split = p.rows == nullptr;
+    const int64_t items = (int64_t)p.n_items * p.num_kv_heads, blocks = split ? items : (items + 7) / 8;
     if (blocks > 0x7fffffff || num_layers > 65535) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)blocks, num_layers);
     if (pool8) return launch_bounds_d<true, __half>(p, head_dim, grid, stream);
