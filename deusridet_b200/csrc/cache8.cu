@@ -107,8 +107,9 @@ struct TokenPlace {
 };
 
 // A CTA takes some tokens, D / 16 lanes per row, two runs of 8 elements a lane: a token's K heads, then its V heads, as in its
-// page block.  The next row is on its way while one is worked on.  Bound by instructions: 30 001 tokens of 4 heads of 256 take
-// 33 us, 5.6 TB/s; one run a lane 41, and without the read ahead, a token a CTA, 77.
+// page block.  The next row is on its way while one is worked on.  30 001 tokens of 4 heads of 256 take 33 us, 5.6 TB/s, with half
+// of the issue slots and of DRAM's cycles busy: bound by the chain through a row's maximum.  One run a lane (more steps in that chain
+// a byte) 41 us, and without the read ahead, a token a CTA, 77.
 constexpr int kAppendRuns = 2;
 struct RowRuns { Vec16 v[kAppendRuns]; };
 template <typename T, int D>

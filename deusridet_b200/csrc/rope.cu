@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 4 : 8) rope
     const bool turns = l < rot_lanes;
     const int live_pairs = half - 4 * l;                        // of the lane's four words, those that turn (not kHalves)
     const bool second = !PAIRS && l >= half_lanes;
+    const uint32_t flip = second ? 0u : 0x80008000u;            // both signs of a word
     const int partner = (threadIdx.x & 31) + (PAIRS || !turns ? 0 : second ? -half_lanes : half_lanes);
     const int trig0 = !turns ? 0 : PAIRS || ANY ? 4 * l : 8 * (second ? l - half_lanes : l);
     const int ring = ring_elements(lanes);
@@ -270,15 +271,12 @@ __global__ void __launch_bounds__(kRopeThreads, MODE == kAnyHalves ? 4 : 8) rope
             float y0, y1;
             if (PAIRS) {
                 rope_pair(own.x, own.y, c[i], s[i], y0, y1);
-            } else if (ANY) {
-                const float2 o = Elem<T>::unpack2(other.w[i]);
+            } else {
+                // first half: x0 c - x1 s; second: x1 c + x0 s (kAnyHalves: the sign is the table's)
+                const uint32_t w = ANY ? other.w[i] : __shfl_sync(0xffffffffu, x.v.w[i], partner) ^ flip;
+                const float2 o = Elem<T>::unpack2(w);
                 y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, s[2 * i]));
                 y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, s[2 * i + 1]));
-            } else {
-                const float2 o = Elem<T>::unpack2(__shfl_sync(0xffffffffu, x.v.w[i], partner));
-                // first half: x0 c - x1 s; second: x1 c + x0 s
-                y0 = __fmaf_rn(own.x, c[2 * i], __fmul_rn(o.x, second ? s[2 * i] : -s[2 * i]));
-                y1 = __fmaf_rn(own.y, c[2 * i + 1], __fmul_rn(o.y, second ? s[2 * i + 1] : -s[2 * i + 1]));
             }
             y.w[i] = (MODE == kHalves ? turns : i < live_pairs) ? Elem<T>::pack2(y0, y1) : x.v.w[i];
         }
