@@ -56,8 +56,8 @@ __device__ __forceinline__ void load_key(const uint8_t* block, const BoundsParam
     }
 }
 
-// One warp per (page, KV head), or a CTA whose warps share the slots (SPLIT: what covers more than a token a page; 2 048
-// tokens of 8 heads of 256 on pages of 128: 9 us, by one warp each 63).  What a launch covers:
+// One warp per (page, KV head), or a CTA whose warps share the slots (SPLIT: what covers more than a token a page and has too
+// few pages to fill the SMs with a warp each; 2 048 of 8 heads of 256 on pages of 128: 9 us, by one warp each 63).  What a launch covers:
 //   rows != null    the page of every batch entry's position, that slot (entries of one sequence in the same page are
 //                   gathered by the first of them: one writer per page)
 //   table != null   the pages of one sequence that hold tokens [pos_start, pos_start + m), those slots
@@ -569,14 +569,14 @@ __global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const Selec
 }
 
 template <bool POOL8, typename T>
-cudaError_t launch_bounds_d(const BoundsParams& p, int head_dim, dim3 grid, cudaStream_t s) {
+cudaError_t launch_bounds_d(const BoundsParams& p, bool split, int head_dim, dim3 grid, cudaStream_t s) {
     switch (head_dim) {
-        case 64: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 64, true>, grid, dim3(256), 0, s, p)
-                                         : launch_pdl(bounds_kernel<POOL8, T, 64, false>, grid, dim3(256), 0, s, p);
-        case 128: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 128, true>, grid, dim3(256), 0, s, p)
-                                         : launch_pdl(bounds_kernel<POOL8, T, 128, false>, grid, dim3(256), 0, s, p);
-        case 256: return p.rows == nullptr ? launch_pdl(bounds_kernel<POOL8, T, 256, true>, grid, dim3(256), 0, s, p)
-                                         : launch_pdl(bounds_kernel<POOL8, T, 256, false>, grid, dim3(256), 0, s, p);
+        case 64: return split ? launch_pdl(bounds_kernel<POOL8, T, 64, true>, grid, dim3(256), 0, s, p)
+                              : launch_pdl(bounds_kernel<POOL8, T, 64, false>, grid, dim3(256), 0, s, p);
+        case 128: return split ? launch_pdl(bounds_kernel<POOL8, T, 128, true>, grid, dim3(256), 0, s, p)
+                              : launch_pdl(bounds_kernel<POOL8, T, 128, false>, grid, dim3(256), 0, s, p);
+        case 256: return split ? launch_pdl(bounds_kernel<POOL8, T, 256, true>, grid, dim3(256), 0, s, p)
+                              : launch_pdl(bounds_kernel<POOL8, T, 256, false>, grid, dim3(256), 0, s, p);
         default: return cudaErrorInvalidValue;
     }
 }
@@ -609,13 +609,14 @@ cudaError_t launch_score(const SelectParams& p, int num_sms, cudaStream_t s) {
 
 cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, cudaStream_t stream) {
     if (p.n_items <= 0 || num_layers <= 0) return cudaSuccess;
-    const bool split = p.rows == nullptr;
-    const int64_t items = (int64_t)p.n_items * p.num_kv_heads, blocks = split ? items : (items + 7) / 8;
+    const int64_t items = (int64_t)p.n_items * p.num_kv_heads;
+    const bool split = p.rows == nullptr && items * num_layers < 64 * 148;   // 64 warps an SM
+    const int64_t blocks = split ? items : (items + 7) / 8;
     if (blocks > 0x7fffffff || num_layers > 65535) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)blocks, num_layers);
-    if (pool8) return launch_bounds_d<true, __half>(p, head_dim, grid, stream);
-    return dtype == DRKV_DTYPE_F16 ? launch_bounds_d<false, __half>(p, head_dim, grid, stream)
-                                   : launch_bounds_d<false, __nv_bfloat16>(p, head_dim, grid, stream);
+    if (pool8) return launch_bounds_d<true, __half>(p, split, head_dim, grid, stream);
+    return dtype == DRKV_DTYPE_F16 ? launch_bounds_d<false, __half>(p, split, head_dim, grid, stream)
+                                   : launch_bounds_d<false, __nv_bfloat16>(p, split, head_dim, grid, stream);
 }
 
 cudaError_t launch_bounds_copy(const BoundsParams& p, int head_dim, int src_page, int dst_page, int num_layers, cudaStream_t stream) {

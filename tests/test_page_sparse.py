@@ -142,6 +142,31 @@ def test_bounds_follow_every_write(drkv_lib, tmp_path, pool, dtype, d, page):
     eng.close()
 
 
+@pytest.mark.parametrize("pool", [None, "e4m3"])
+def test_bounds_of_a_long_chunk(drkv_lib, pool):
+    """So many pages that a warp takes one each, begun inside a page; appended, then scanned."""
+    import torch
+    n, hkv, d, page = 19203, 8, 64, 16
+    eng = _engine(pool, 8, hkv, d, page, "bf16", 1210, 1, 1205)
+    eng.page_bounds_enable()
+    _start(eng, [n])
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k = _rows(n, hkv, d, torch.bfloat16, g)
+    eng.append_rope_chunk(0, 0, 0, 5, k[:5].contiguous(), k[:5].contiguous())
+    eng.append_rope_chunk(0, 0, 5, n - 5, k[5:].contiguous(), k[5:].contiguous())
+    torch.cuda.synchronize()
+    ks = _stored(k, pool)
+    _check_bounds(eng, 0, 0, ks, page)
+    bounds, exponents = eng.page_bounds()
+    bounds.zero_()
+    exponents.zero_()
+    eng.page_bounds_enable()
+    torch.cuda.synchronize()
+    _check_bounds(eng, 0, 0, ks[:n // page * page], page)
+    eng.check_kernels()
+    eng.close()
+
+
 def test_bounds_of_extreme_keys(drkv_lib):
     """Zeros, the smallest and largest values, infinities and NaN."""
     import torch
