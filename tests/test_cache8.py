@@ -290,6 +290,78 @@ def test_decode_against_64_bits(drkv_lib, dtype, d, grp, hkv, page):
 
 
 @pytest.mark.gpu
+def test_one_long_call_and_many_short_ones(drkv_lib):
+    """Appends, flat copies out and in: the same bytes whether a CTA takes one token or a hundred."""
+    import torch
+    n, d = 90001, 128
+    one, many = (_engine(hq=1, hkv=1, d=d, page=16, dtype="bf16", pages=5700, seqs=1, per_seq=5700, rot=32) for _ in range(2))
+    for e in (one, many):
+        e.seq_create()
+        assert e.ensure_blocks_for_range(0, 0, n)
+        e.set_seq_len(0, n)
+        e.sync_block_table()
+        e.pool_tensor().zero_()
+    g = torch.Generator(device="cuda").manual_seed(12)
+    k, v = (torch.randn(n, 1, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    one.append_rope_chunk(0, 0, 0, n, k, v)
+    for a in range(0, n, 701):
+        b = min(n, a + 701)
+        many.append_rope_chunk(0, 0, a, b - a, k[a:b].contiguous(), v[a:b].contiguous())
+    torch.cuda.synchronize()
+    assert torch.equal(one.pool_tensor(), many.pool_tensor())
+    flat = torch.empty(1, 2, n, 1, d, device="cuda", dtype=torch.bfloat16)
+    one.extract(0, 0, n, flat)
+    for a in range(0, n, 14001):
+        b = min(n, a + 14001)
+        part = torch.empty(1, 2, b - a, 1, d, device="cuda", dtype=torch.bfloat16)
+        many.extract(0, a, b - a, part)
+        torch.cuda.synchronize()
+        assert torch.equal(part, flat[:, :, a:b])
+    one.pool_tensor().zero_()
+    one.inject(0, 0, n, flat)
+    many.pool_tensor().zero_()
+    for a in range(0, n, 14001):
+        b = min(n, a + 14001)
+        many.inject(0, a, b - a, flat[:, :, a:b].contiguous())
+    torch.cuda.synchronize()
+    assert torch.equal(one.pool_tensor(), many.pool_tensor())
+    # A stored row quantises to the values it has, if not to its bytes: a maximum between 224 and 232 times 2^e was rounded to
+    # 224 * 2^e = 448 * 2^(e - 1), and then e - 1 with doubled codes holds the same row.
+    again = torch.empty_like(flat)
+    one.extract(0, 0, n, again)
+    torch.cuda.synchronize()
+    assert torch.equal(again, flat)
+    one.close()
+    many.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_seq,grp,hkv,d", [(1, 4, 1, 256), (6, 8, 2, 128), (16, 8, 2, 128), (12, 8, 2, 128), (40, 8, 2, 128), (5, 16, 1, 256),
+                                             (37, 16, 1, 256), (20, 4, 8, 64), (300, 4, 2, 64)])
+def test_pieces_of_every_number(drkv_lib, n_seq, grp, hkv, d):
+    """From hundreds of pieces a row to two, few rows and many: every way of merging them; entries of one table row."""
+    import torch
+    n = 1900
+    eng = _engine(hq=grp * hkv, hkv=hkv, d=d, page=16, dtype="bf16", pages=128, seqs=1, per_seq=120)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, n)
+    eng.set_seq_len(0, n)
+    eng.sync_block_table()
+    stored = _fill(eng, [n], "bf16", 9, spread=1)[0]
+    g = torch.Generator(device="cuda").manual_seed(n_seq)
+    lens = [n - 37 * (i % 40) - i % 16 for i in range(n_seq)]
+    q = torch.randn(n_seq, grp * hkv, d, generator=g, device="cuda").bfloat16()
+    out = torch.full_like(q, 7.0)
+    rows = torch.zeros(n_seq, device="cuda", dtype=torch.int32)
+    eng.attend_decode(0, n_seq, rows, torch.tensor(lens, device="cuda", dtype=torch.int32), n, q, out, 1.0 / math.sqrt(d))
+    torch.cuda.synchronize()
+    eng.check_kernels()
+    some = sorted(set(range(0, n_seq, max(1, n_seq // 12))) | {n_seq - 1})
+    _check_decode(out[some], out[some], q[some], [stored for _ in some], [lens[i] for i in some], hkv, 1.0 / math.sqrt(d), "bf16")
+    eng.close()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_values_of_unlike_size(drkv_lib, dtype):
     """One value row is 2^20 times the others and has next to no weight; one query row is tiny, one large."""
