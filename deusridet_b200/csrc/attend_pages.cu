@@ -21,9 +21,13 @@
 // rows would be half empty.  P turns from the accumulator layout into the operand layout by movmatrix.  e4m3 operands
 // become f16 two at a time (cvt.rn.f16x2.e4m3x2, exact).
 //
-// Scales of the 8-bit rows stay exponents.  K's multiply the score.  V's multiply the weight: with E the largest exponent
-// seen so far, weights are p * 2^(ev - E + 7) in f16, at most 2^15 since p may reach 2^8 before the maximum follows, and of
-// full precision down to 2^-21 of the largest; o carries 2^E.
+// Scales of the 8-bit rows stay exponents.  K's multiply the score.  V's join the weight: what a key adds to o is
+// 2^(s + ev) times its bytes (s in the log2 domain), and f16 has 40 binades for the weights of all keys.  So weights have a
+// reference of their own beside the softmax's maximum m, per head: E such that m + E is the largest s + ev seen so far.  They
+// are 2^((s - m) + (ev - E) + 7), at most 2^15 since they may pass the reference by 2^8 before it follows, of full precision
+// down to 2^-20 of the largest, and vanish below 2^-31 of it: next to what the same head has summed, whatever the sizes of
+// rows that hold no weight.  o carries 2^E, in the pieces too; the sum of the weights stays relative to m, in fp32.
+// (A second exponential and two additions per key and head: 64 sequences, 109.8 us a step with them and without.)
 // bf16 queries are scaled by a power of two per head into f16 (8 significant bits fit; exact unless an element is below
 // 2^-27 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
 // P in the PV product: f16 hi + lo terms (22 bits) where the output is f16, bf16 hi + lo (16 bits) for a bf16 pool,
@@ -57,6 +61,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
+// An exponent byte that is no less than x; 2^(byte - 127) is finite.
+__device__ __forceinline__ float whole_byte(float x) { return fminf(fmaxf(ceilf(x), 0.f), 254.f); }
+
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <>
@@ -78,13 +85,13 @@ struct Split {
 constexpr size_t kSplitFloats = sizeof(Split) / 4;
 
 // Pieces: slot = 2 * warp + (the stretch begins inside the pair ? 0 : 1), row = slot * group + head of the group;
-// un-normalised sums [row][D], then maxima (log2 domain) and sums of weights as pairs [row].
+// un-normalised sums [row][D], then (maximum in the log2 domain, sum of weights, exponent byte that o is relative to, 0) [row].
 struct Pieces {
     float* o;
-    float2* ml;
+    float4* mle;
     __host__ __device__ Pieces(float* scratch, int n_warps, int group, int d) {
         o = scratch + kSplitFloats;
-        ml = reinterpret_cast<float2*>(o + 2 * (size_t)n_warps * group * d);
+        mle = reinterpret_cast<float4*>(o + 2 * (size_t)n_warps * group * d);
     }
 };
 
@@ -275,7 +282,8 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
     uint32_t qf[NQ][KSTEPS][2];
     float qs[NQ][2];                                                        // score factor of heads 2t and 2t + 1
     float o[NQ][MT][4], m[NQ][2], l[NQ][2];
-    int big_e = 0, cur_pair = -1;                                           // big_e: V exponent byte the weights are relative to
+    float lift[NQ][2];                                                      // 8-bit pool: WS - E, E in exponent bytes, whole
+    int cur_pair = -1;
 
     auto begin_pair = [&](int pair) {
         cur_pair = pair;
@@ -333,10 +341,10 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             qs[nq][1] = __shfl_sync(FULL, own_scale, 8 * t + 4);
             m[nq][0] = m[nq][1] = kNoKey;
             l[nq][0] = l[nq][1] = 0.f;
+            lift[nq][0] = lift[nq][1] = WS;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) o[nq][mt][0] = o[nq][mt][1] = o[nq][mt][2] = o[nq][mt][3] = 0.f;
         }
-        big_e = 0;
     };
 
     const Pieces pieces(p.scratch, n_warps, p.group, D);
@@ -346,7 +354,6 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
         const int start = cum[b] + h * groups;
         const bool whole = start >= lo && start + groups <= lo + n;
         const int64_t row0 = (2 * (int64_t)gw + (start > lo ? 1 : 0)) * p.group;
-        const float unit = POOL8 ? exp2_int(big_e - 127) : 1.f;
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -358,7 +365,8 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                 const int head = nq * 8 + 2 * t + c;
                 if (head < p.group) {
                     const float f = (whole ? 1.f / sum : 1.f) * (F16 ? 0x1p-7f : 1.f);
-                    if (!whole && g == 0) pieces.ml[row0 + head] = make_float2(m[nq][c], sum);
+                    const float e = POOL8 ? WS - lift[nq][c] : 127.f, unit = whole ? exp2_int((int)e - 127) : 1.f;
+                    if (!whole && g == 0) pieces.mle[row0 + head] = make_float4(m[nq][c], sum, e, 0.f);
 #pragma unroll
                     for (int j = 0; j < VCH; j++) {
                         const int dim = (g + 8 * j) * EPL;
@@ -423,21 +431,20 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             for (int k = 0; k < 4; k++) s[0][k] += s2[k];
         }
         // s becomes the score in the log2 domain.  A K row whose byte is 0 (everything below 2^-118) counts as zeros.
-        uint32_t ev0 = 0, ev1 = 0;
-        float ks0 = 1.f, ks1 = 1.f;
+        float ev0 = 0.f, ev1 = 0.f, ks0 = 1.f, ks1 = 1.f;
         if (POOL8) {
             ks0 = __uint_as_float(lds8(tile + 2 * TILE + g) << 23);
             ks1 = __uint_as_float(lds8(tile + 2 * TILE + g + 8) << 23);
-            ev0 = lds8(tile + 2 * TILE + 16 + g);
-            ev1 = lds8(tile + 2 * TILE + 24 + g);
+            ev0 = (float)lds8(tile + 2 * TILE + 16 + g);
+            ev1 = (float)lds8(tile + 2 * TILE + 24 + g);
         }
         if (valid < 16) {                                                   // what lies behind the last key may be anything
-            if (g >= valid) ev0 = 0, ks0 = 0.f;
-            if (g + 8 >= valid) ev1 = 0, ks1 = 0.f;
+            if (g >= valid) ev0 = ks0 = 0.f;
+            if (g + 8 >= valid) ev1 = ks1 = 0.f;
         }
-        // The maximum follows only when a score exceeds it by more than kSlack, and then in full: most groups need no
-        // reduction over the lanes.
-        bool grow = (int)max(ev0, ev1) > big_e;
+        // The maximum and the weights' reference follow only when a score exceeds one of them by more than kSlack, and then
+        // in full: most groups need no reduction over the lanes.
+        bool grow = false;
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -447,24 +454,35 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                 // product's lower half alone could exceed the slack
                 s[nq][c] = __fmul_rn(s[nq][c], f0);
                 s[nq][2 + c] = __fmul_rn(s[nq][2 + c], f1);
-                grow |= __fadd_rn(fmaxf(s[nq][c], s[nq][2 + c]), -m[nq][c]) > kSlack;
+                if (POOL8) {
+                    const float t0 = __fadd_rn(s[nq][c], -m[nq][c]), t1 = __fadd_rn(s[nq][2 + c], -m[nq][c]);
+                    grow |= fmaxf(t0, t1) > kSlack;
+                    grow |= fmaxf(t0 + (ev0 + lift[nq][c]), t1 + (ev1 + lift[nq][c])) > kSlack + WS;
+                } else {
+                    grow |= __fadd_rn(fmaxf(s[nq][c], s[nq][2 + c]), -m[nq][c]) > kSlack;
+                }
             }
         if (__any_sync(FULL, grow)) {
-            const int new_e = POOL8 ? max(big_e, __reduce_max_sync(FULL, (int)max(ev0, ev1))) : 0;
-            // 2^(old - new E) in two factors: the difference may be 247
-            const int de = big_e - new_e;
-            const float e1 = exp2_int(max(de, -126)), e2 = exp2_int(max(de - max(de, -126), -126));
-            big_e = new_e;
+            auto over_keys = [&](float a, float b) -> float {               // maximum over the group's visible keys
+                float x = fmaxf(g < valid ? a : -INFINITY, g + 8 < valid ? b : -INFINITY);
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
+                return fmaxf(x, __shfl_xor_sync(FULL, x, 16));
+            };
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    float x = fmaxf(g < valid ? s[nq][c] : -INFINITY, g + 8 < valid ? s[nq][2 + c] : -INFINITY);
-                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(FULL, x, 16));
-                    x = fmaxf(x, m[nq][c]);
-                    const float f = fast_exp2(m[nq][c] - x), r = POOL8 ? f * e1 * e2 : f;
+                    const float x = fmaxf(over_keys(s[nq][c], s[nq][2 + c]), m[nq][c]), down = m[nq][c] - x;
+                    const float f = fast_exp2(down);
+                    float r = f;
+                    if (POOL8) {
+                        // whole, so that o's unit stays a power of two; never above the largest exponent byte met
+                        const float seen = over_keys((s[nq][c] - x) + ev0, (s[nq][2 + c] - x) + ev1), old = WS - lift[nq][c];
+                        const float e = whole_byte(fmaxf(seen, down + old));
+                        r = fast_exp2(down + (old - e));
+                        lift[nq][c] = WS - e;
+                    }
                     m[nq][c] = x;
                     l[nq][c] *= f;
 #pragma unroll
@@ -474,30 +492,22 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                     }
                 }
         }
-        // ---- weights ----
-        float vs0 = F16 ? 0x1p7f : 1.f, vs1 = vs0;
-        if (POOL8) {                                                        // 2^(ev - E + WS), 0 below 2^-126
-            vs0 = __uint_as_float((uint32_t)max((int)ev0 - big_e + WS + 127, 0) << 23);
-            vs1 = __uint_as_float((uint32_t)max((int)ev1 - big_e + WS + 127, 0) << 23);
-        }
+        // ---- weights: p for the sum, w for the product ----
         uint32_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
             float w0[2], w1[2];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                w0[c] = fast_exp2(__fadd_rn(s[nq][c], -m[nq][c]));
-                w1[c] = fast_exp2(__fadd_rn(s[nq][2 + c], -m[nq][c]));
+                const float t0 = __fadd_rn(s[nq][c], -m[nq][c]), t1 = __fadd_rn(s[nq][2 + c], -m[nq][c]);
+                const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
+                l[nq][c] += (g < valid ? p0 : 0.f) + (g + 8 < valid ? p1 : 0.f);
+                w0[c] = POOL8 ? fast_exp2(t0 + (ev0 + lift[nq][c])) : F16 ? p0 * 0x1p7f : p0;
+                w1[c] = POOL8 ? fast_exp2(t1 + (ev1 + lift[nq][c])) : F16 ? p1 * 0x1p7f : p1;
             }
             if (valid < 16) {
                 if (g >= valid) w0[0] = w0[1] = 0.f;
                 if (g + 8 >= valid) w1[0] = w1[1] = 0.f;
-            }
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                l[nq][c] += w0[c] + w1[c];
-                w0[c] *= vs0;
-                w1[c] *= vs1;
             }
             const uint32_t h0 = Elem<TM>::pack2(w0[0], w0[1]), h1 = Elem<TM>::pack2(w1[0], w1[1]);
             pf[nq][0] = transpose8x8(h0);
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(CTA_DIMS ? 256 : 128, 1) merge_pieces_kernel(c
     constexpr int DIMS = WIDE ? CTA_DIMS : D, LANES = DIMS / 4;
     constexpr int PARTS = WIDE ? 256 / LANES : 1, ROWS = WIDE ? 1 : 128 / LANES;
     __shared__ float4 s_o[WIDE ? PARTS : 1][LANES];
-    __shared__ float2 s_ml[WIDE ? PARTS : 1];
+    __shared__ float4 s_mle[WIDE ? PARTS : 1];
     pdl_wait();
     pdl_launch_dependents();
     const Split* split = reinterpret_cast<const Split*>(p.scratch);
@@ -606,65 +616,78 @@ __global__ void __launch_bounds__(CTA_DIMS ? 256 : 128, 1) merge_pieces_kernel(c
     const int64_t step = 2 * p.group, row1 = 2 * (int64_t)first * p.group + head;   // piece i > 0 at row1 + i * step
     const int64_t row0 = row1 + (start != first * share ? p.group : 0);
     const float* o = pieces.o + (WIDE ? blockIdx.y * DIMS : 0) + 4 * d4;
-    float m = kNoKey, l = 0.f;
+    float m = kNoKey, l = 0.f, e = 0.f;                                     // e: exponent byte that acc is relative to
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (n >= 2) {
 #pragma unroll 1
         for (int i0 = part; i0 < n; i0 += 8 * PARTS) {
-            float2 ml[8];
-            float4 x[8];
+            float4 mle[8], x[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int i = i0 + k * PARTS;
                 const int64_t r = i ? row1 + i * step : row0;
-                ml[k] = make_float2(kNoKey, 0.f);
+                mle[k] = make_float4(kNoKey, 0.f, 0.f, 0.f);
                 x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (i < n) {
-                    ml[k] = __ldcg(pieces.ml + r);
+                    mle[k] = __ldcg(pieces.mle + r);
                     x[k] = __ldcg(reinterpret_cast<const float4*>(o + r * D));
                 }
             }
             float top = m;
 #pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, ml[k].x);
-            const float f0 = fast_exp2(m - top);
+            for (int k = 0; k < 8; k++) top = fmaxf(top, mle[k].x);
+            float e_top = (m - top) + e;
+#pragma unroll
+            for (int k = 0; k < 8; k++) e_top = fmaxf(e_top, (mle[k].x - top) + mle[k].z);
+            e_top = whole_byte(e_top);
+            l *= fast_exp2(m - top);
+            const float f0 = fast_exp2((m - top) + (e - e_top));
             m = top;
-            l *= f0;
+            e = e_top;
             acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                const float f = fast_exp2(ml[k].x - top);                   // absent: 2^(no key - top) * 0
-                l += ml[k].y * f;
+                const float down = mle[k].x - top, f = fast_exp2(down + (mle[k].z - e_top));   // absent: acc stays, 2^.. * 0
+                l += mle[k].y * fast_exp2(down);
                 acc.x += x[k].x * f, acc.y += x[k].y * f, acc.z += x[k].z * f, acc.w += x[k].w * f;
             }
         }
     }
     if (WIDE) {
         s_o[set][d4] = acc;
-        if (d4 == 0) s_ml[set] = make_float2(m, l);
+        if (d4 == 0) s_mle[set] = make_float4(m, l, e, 0.f);
         __syncthreads();
-        if (set != 0) return;
-        float top = m;
-#pragma unroll 1
-        for (int i = 1; i < PARTS; i++) top = fmaxf(top, s_ml[i].x);
-        const float f0 = fast_exp2(m - top);
-        l *= f0;
-        acc.x *= f0, acc.y *= f0, acc.z *= f0, acc.w *= f0;
+        if (threadIdx.x >= (LANES > 32 ? LANES : 32)) return;
+        // lane i of every warp left works out set i's factors; the sets are added in their order
+        const int lane = threadIdx.x & 31;
+        const float4 st = lane < PARTS ? s_mle[lane] : make_float4(kNoKey, 0.f, 0.f, 0.f);
+        float top = st.x;
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+        const float down = st.x - top;
+        float e_top = down + st.z;
+#pragma unroll
+        for (int i = 1; i < 32; i <<= 1) e_top = fmaxf(e_top, __shfl_xor_sync(0xffffffffu, e_top, i));
+        e = whole_byte(e_top);
+        const float fl = fast_exp2(down), fo = fast_exp2(down + (st.z - e));
+        l = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int i = 1; i < PARTS; i++) {
-            const float f = fast_exp2(s_ml[i].x - top);
+        for (int i = 0; i < PARTS; i++) {
+            const float f = __shfl_sync(0xffffffffu, fo, i);
             const float4 x = s_o[i][d4];
-            l += s_ml[i].y * f;
+            l += __shfl_sync(0xffffffffu, st.y, i) * __shfl_sync(0xffffffffu, fl, i);
             acc.x += x.x * f, acc.y += x.y * f, acc.z += x.z * f, acc.w += x.w * f;
         }
+        if (set != 0) return;
     } else if (n < 2) {
         return;
     }
     if (!(l != 0.f)) return;                                                // no visible key: the row stays as it is
-    const float inv = 1.f / l;
+    const float inv = 1.f / l, unit = exp2_int((int)e - 127);
     uint2 v;
-    v.x = Elem<T>::pack2(acc.x * inv, acc.y * inv);
-    v.y = Elem<T>::pack2(acc.z * inv, acc.w * inv);
+    v.x = Elem<T>::pack2(acc.x * inv * unit, acc.y * inv * unit);
+    v.y = Elem<T>::pack2(acc.z * inv * unit, acc.w * inv * unit);
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + (int64_t)row * D + (WIDE ? blockIdx.y * DIMS : 0) + 4 * d4) = v;
 }
 
@@ -719,7 +742,7 @@ cudaError_t launch_group(const AttendPagesParams& p, bool pool8, int num_sms, cu
 
 size_t attend_pages_scratch_bytes(int group, int head_dim, int num_sms) {
     const size_t rows = 2 * (size_t)num_sms * 16 * group;                  // at most 16 warps a CTA
-    return (kSplitFloats + rows * (head_dim + 2)) * sizeof(float);
+    return (kSplitFloats + rows * (head_dim + 4)) * sizeof(float);
 }
 
 cudaError_t launch_attend_pages(const AttendPagesParams& p, bool pool8, int head_dim, int dtype, int num_sms, cudaStream_t stream) {
