@@ -30,8 +30,8 @@
 // (A second exponential and two additions per key and head: 64 sequences, 109.8 us a step with them and without.)
 // bf16 queries are scaled by a power of two per head into f16 (8 significant bits fit; exact unless an element is below
 // 2^-27 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
-// P in the PV product: f16 hi + lo terms (22 bits) where the output is f16, bf16 hi + lo (16 bits) for a bf16 pool,
-// one f16 term (2^-11) where the pool is 8-bit and the output bf16 (2^-8 steps).
+// P in the PV product: f16 hi + lo terms (22 bits) over an 8-bit or an f16 pool, bf16 hi + lo (16 bits) over a bf16 pool.  (One
+// f16 term for bf16 outputs of the 8-bit pool took as long: 109.8 us for 64 sequences with one, 108.7 with two.)
 #include <atomic>
 
 #include "kernels.hpp"
@@ -114,7 +114,6 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
     constexpr int WARPS = Ring<POOL8, D, NQ>::kWarps, STAGES = Ring<POOL8, D, NQ>::kStages, THREADS = WARPS * 32;
     using TM = typename std::conditional<POOL8, __half, T>::type;           // matrix operand type
     constexpr bool F16 = std::is_same<TM, __half>::value;
-    constexpr bool LO = !(POOL8 && std::is_same<T, __nv_bfloat16>::value);
     constexpr int ROWB = D * (POOL8 ? 1 : 2), CPR = ROWB / 16, TILE = 16 * ROWB;
     constexpr int SLOT = 2 * TILE + (POOL8 ? 32 : 0);
     constexpr int KSTEPS = D / 16, MT = D / 16;
@@ -512,11 +511,9 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             const uint32_t h0 = Elem<TM>::pack2(w0[0], w0[1]), h1 = Elem<TM>::pack2(w1[0], w1[1]);
             pf[nq][0] = transpose8x8(h0);
             pf[nq][1] = transpose8x8(h1);
-            if (LO) {
-                const float2 a = Elem<TM>::unpack2(h0), b = Elem<TM>::unpack2(h1);
-                pl[nq][0] = transpose8x8(Elem<TM>::pack2(w0[0] - a.x, w0[1] - a.y));
-                pl[nq][1] = transpose8x8(Elem<TM>::pack2(w1[0] - b.x, w1[1] - b.y));
-            }
+            const float2 a = Elem<TM>::unpack2(h0), b = Elem<TM>::unpack2(h1);
+            pl[nq][0] = transpose8x8(Elem<TM>::pack2(w0[0] - a.x, w0[1] - a.y));
+            pl[nq][1] = transpose8x8(Elem<TM>::pack2(w1[0] - b.x, w1[1] - b.y));
         }
         // ---- O^T += V^T P^T: keys 2t, 2t + 1, 2t + 8, 2t + 9; dims (g + 8 j) EPL + 0 .. EPL - 1 ----
         const uint32_t vt = tile + TILE;
@@ -524,7 +521,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++) {
                 mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pf[nq][0], pf[nq][1]);
-                if (LO) mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pl[nq][0], pl[nq][1]);
+                mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pl[nq][0], pl[nq][1]);
             }
         };
 #pragma unroll

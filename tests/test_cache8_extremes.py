@@ -103,3 +103,29 @@ def test_weight_on_a_row_of_nothing(drkv_lib, n, n_seq, d):
             assert (err <= tol).all(), (sink, rest, b, float((err / tol).max()))
     eng.check_kernels()
     eng.close()
+
+
+@pytest.mark.parametrize("n,d,grp", [(2, 128, 4), (5, 64, 9), (40, 256, 2), (900, 128, 8)])
+def test_weights_of_bf16_outputs(drkv_lib, n, d, grp):
+    """Weights go into the product with 22 bits whatever the output's type: what is off is the output's rounding."""
+    import torch
+    eng = _engine(hq=grp, hkv=1, d=d, page=16, dtype="bf16", pages=64, seqs=1)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, n)
+    eng.set_seq_len(0, n)
+    eng.sync_block_table()
+    g = torch.Generator(device="cuda").manual_seed(n)
+    k, v = (torch.randn(n, 1, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    q = torch.randn(150, grp, d, generator=g, device="cuda").bfloat16()
+    eng.append_rope_chunk(0, 0, 0, n, k, v)
+    kv_len = torch.full((150,), n, device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 7.0)
+    eng.attend_decode(0, 150, torch.zeros_like(kv_len), kv_len, n, q, out, 0.5 / math.sqrt(d))
+    torch.cuda.synchronize()
+    ks, vs = (R.stored_values(x.double().cpu().numpy())[:, 0] for x in (k, v))
+    got, qd = out.double().cpu().numpy(), q.double().cpu().numpy()
+    for b in range(150):
+        want, pv, mag = R.attend(qd[b], ks, vs, 0.5 / math.sqrt(d))
+        assert (np.abs(got[b] - want) <= R.attend_tolerance(want, pv, mag, _half_step("bf16"), 2.0 ** -21)).all(), b
+    eng.check_kernels()
+    eng.close()
