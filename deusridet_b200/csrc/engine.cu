@@ -1115,11 +1115,28 @@ static int decode_common(drkv_engine* e, int layer, int n_seq, const int32_t* d_
     return DRKV_OK;
 }
 
+// What attend_pages refuses, and how many sequences one of its launches takes; a call that writes before it attends asks first.
+static int attend_pages_step(drkv_engine* e, int max_kv_len, int list_len, const void* q, const void* out, int* step) {
+    if (!aligned16(q, out)) return set_err(DRKV_ERR_INVALID, "attend: q and out must be 16-byte aligned");
+    const drkv_geometry& g = e->geom;
+    const int64_t row_tokens = (int64_t)e->book.row_width() * g.page_size;
+    if (max_kv_len > row_tokens) max_kv_len = (int)row_tokens;
+    // the kernel counts 16-key groups of a launch in 32 bits
+    int64_t groups = ((int64_t)max_kv_len + 15) / 16;
+    if (list_len > 0 && (int64_t)list_len * (g.page_size / 16) < groups) groups = (int64_t)list_len * (g.page_size / 16);
+    const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxPagesSeqs;
+    if (cap < 1) return set_err(DRKV_ERR_CAPACITY, "attend: %d keys of %d KV heads are more than one launch takes", max_kv_len, g.num_kv_heads);
+    *step = cap < kMaxPagesSeqs ? (int)cap : kMaxPagesSeqs;
+    return DRKV_OK;
+}
+
 // Decode attention over the 8-bit pool, and over listed pages of either pool (attend_pages.cu).
 static int attend_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
                         const int32_t* d_list, int list_len, const void* q, void* out, float scale, cudaStream_t stream) {
     const drkv_geometry& g = e->geom;
-    if (!aligned16(q, out)) return set_err(DRKV_ERR_INVALID, "attend: q and out must be 16-byte aligned");
+    int step = 0;
+    int rc = attend_pages_step(e, max_kv_len, d_list ? list_len : 0, q, out, &step);
+    if (rc != DRKV_OK) return rc;
     DeviceGuard dev(e->device);
     note_stream(e, stream);
     const int64_t row_tokens = (int64_t)e->book.row_width() * g.page_size;
@@ -1142,12 +1159,6 @@ static int attend_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_r
     p.scale_log2 = scale * 1.4426950408889634f;
     p.scratch = e->d_scratch;
     p.error_word = e->d_error;
-    // the kernel counts 16-key groups of a launch in 32 bits
-    int64_t groups = ((int64_t)max_kv_len + 15) / 16;
-    if (d_list && (int64_t)list_len * (g.page_size / 16) < groups) groups = (int64_t)list_len * (g.page_size / 16);
-    const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxPagesSeqs;
-    if (cap < 1) return set_err(DRKV_ERR_CAPACITY, "attend: %d keys of %d KV heads are more than one launch takes", max_kv_len, g.num_kv_heads);
-    const int step = cap < kMaxPagesSeqs ? (int)cap : kMaxPagesSeqs;
     const size_t row_bytes = (size_t)g.num_q_heads * g.head_dim * 2;
     for (int s0 = 0; s0 < n_seq; s0 += step) {
         p.n_seq = n_seq - s0 < step ? n_seq - s0 : step;
@@ -1191,8 +1202,11 @@ int drkv_attend_decode(drkv_engine* e, int layer, int n_seq, const int32_t* d_ro
 // The decode step over the 8-bit pool: the append is a launch of its own (positions d_kv_len - 1).
 static int append_attend8(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len, int max_kv_len,
                           const void* k_src, const void* v_src, const void* q, void* out, float scale, cudaStream_t stream) {
+    int step = 0;
+    int rc = attend_pages_step(e, max_kv_len, 0, q, out, &step);     // a refused call leaves the cache as it was
+    if (rc != DRKV_OK) return rc;
     DeviceGuard dev(e->device);
-    int rc = append8(e, layer, n_seq, d_rows, d_kv_len, 0, -1, k_src, v_src, stream);
+    rc = append8(e, layer, n_seq, d_rows, d_kv_len, 0, -1, k_src, v_src, stream);
     if (rc == DRKV_OK) rc = widen_batch(e, layer, n_seq, d_rows, d_kv_len, -1, stream);
     return rc == DRKV_OK ? attend_pages(e, layer, n_seq, d_rows, d_kv_len, max_kv_len, nullptr, 0, q, out, scale, stream) : rc;
 }

@@ -129,3 +129,33 @@ def test_weights_of_bf16_outputs(drkv_lib, n, d, grp):
         assert (np.abs(got[b] - want) <= R.attend_tolerance(want, pv, mag, _half_step("bf16"), 2.0 ** -21)).all(), b
     eng.check_kernels()
     eng.close()
+
+
+def test_refused_steps_leave_the_cache(drkv_lib):
+    """A decode step with a bad pointer writes no token and widens no bounds, by batch and by plan."""
+    import torch
+    from deusridet_b200 import DrkvError, capi
+    eng = _engine(hq=8, hkv=2, d=128, page=16, dtype="bf16", pages=8, seqs=1)
+    eng.page_bounds_enable()
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, 20)
+    eng.set_seq_len(0, 20)
+    eng.sync_block_table()
+    eng.pool_tensor().zero_()
+    eng.page_bounds_enable()
+    x = torch.ones(2, 8, 128, device="cuda", dtype=torch.bfloat16)
+    rows, kv_len = torch.zeros(1, device="cuda", dtype=torch.int32), torch.full((1,), 20, device="cuda", dtype=torch.int32)
+    eng.plan_decode([0], [20])
+    before = [t.clone() for t in (eng.pool_tensor(), *eng.page_bounds())]
+    off = x.data_ptr() + 4
+    for ptrs in ((x, x, x, off), (x, x, off, x), (off, x, x, x), (x, off, x, x)):
+        for call in (lambda: eng.append_attend_decode(0, 1, rows, kv_len, 20, *ptrs, 1.0), lambda: eng.append_attend_decode_planned(0, *ptrs, 1.0)):
+            with pytest.raises(DrkvError) as err:
+                call()
+            assert err.value.code == capi.ERR_INVALID
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(before, (eng.pool_tensor(), *eng.page_bounds())))
+    eng.append_attend_decode(0, 1, rows, kv_len, 20, x, x, x, torch.empty_like(x), 1.0)
+    torch.cuda.synchronize()
+    assert not torch.equal(before[0], eng.pool_tensor()) and not torch.equal(before[1], eng.page_bounds()[0])
+    eng.close()
