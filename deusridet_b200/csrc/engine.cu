@@ -1123,7 +1123,10 @@ static int attend_pages_step(drkv_engine* e, int max_kv_len, int list_len, const
     if (max_kv_len > row_tokens) max_kv_len = (int)row_tokens;
     // the kernel counts 16-key groups of a launch in 32 bits
     int64_t groups = ((int64_t)max_kv_len + 15) / 16;
-    if (list_len > 0 && (int64_t)list_len * (g.page_size / 16) < groups) groups = (int64_t)list_len * (g.page_size / 16);
+    if (list_len > 0) {                                              // whole pages there, the last one too
+        const int64_t pages = ((int64_t)max_kv_len + g.page_size - 1) / g.page_size;
+        groups = (pages < list_len ? pages : list_len) * (g.page_size / 16);
+    }
     const int64_t cap = groups > 0 ? (1ll << 30) / (groups * g.num_kv_heads) : kMaxPagesSeqs;
     if (cap < 1) return set_err(DRKV_ERR_CAPACITY, "attend: %d keys of %d KV heads are more than one launch takes", max_kv_len, g.num_kv_heads);
     *step = cap < kMaxPagesSeqs ? (int)cap : kMaxPagesSeqs;

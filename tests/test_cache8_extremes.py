@@ -159,3 +159,30 @@ def test_refused_steps_leave_the_cache(drkv_lib):
     torch.cuda.synchronize()
     assert not torch.equal(before[0], eng.pool_tensor()) and not torch.equal(before[1], eng.page_bounds()[0])
     eng.close()
+
+
+def test_lists_over_one_vast_page(drkv_lib):
+    """A list counts whole pages: 1 024 sequences of twenty keys on a page of 2^25 tokens are 2^31 groups of 16, more than a
+    launch counts."""
+    import torch
+    from deusridet_b200 import PagedKVEngine
+    eng = PagedKVEngine(num_layers=1, num_q_heads=1, num_kv_heads=1, head_dim=64, page_size=2 ** 25, dtype="f16", rotary_dim=0,
+                        max_pages=4, max_seqs=1, max_pages_per_seq=1, device=0)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, 20)
+    eng.set_seq_len(0, 20)
+    eng.sync_block_table()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(20, 1, 64, generator=g, device="cuda").half() for _ in range(2))
+    q = torch.randn(1024, 1, 64, generator=g, device="cuda").half()
+    eng.append_rope_chunk(0, 0, 0, 20, k, v)
+    kv_len = torch.full((1024,), 20, device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 7.0)
+    zeros = torch.zeros_like(kv_len)
+    eng.attend_selected(0, 1024, zeros, kv_len, 20, zeros, 1, q, out, 0.125)
+    torch.cuda.synchronize()
+    eng.check_kernels()
+    kd, vd, qd, got = (x.double().cpu().numpy() for x in (k[:, 0], v[:, 0], q[:, 0], out[:, 0]))
+    want, pv, mag = R.attend(qd, kd, vd, 0.125)
+    assert (np.abs(got - want) <= R.attend_tolerance(want, pv, mag, _half_step("f16"), 2.0 ** -21)).all()
+    eng.close()
