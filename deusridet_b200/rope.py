@@ -75,13 +75,17 @@ class Rope:
     def apply(self, pos, q=None, k=None, *, out_q=None, out_k=None, inverse: bool = False, stream=None):
         """Rotates q and k, tensors [n_tokens, heads, head_dim] of any token and head strides, by the int32 positions
         `pos` [n_tokens]; into out_q / out_k (new contiguous tensors by default; the input itself for in place).
-        inverse=True applies the transpose, the gradient.  Runs on `stream`, by default the device's current one; new outputs
+        inverse=True applies the transpose, the gradient; apply itself is not recorded for autograd, tensors that require one
+        are refused while gradients are enabled.  Runs on `stream`, by default the device's current one; new outputs
         belong to it.  Returns (out_q, out_k)."""
         import torch
         if q is None and k is None:
             raise ValueError("nothing to rotate: give q, k or both")
         if (q is None and out_q is not None) or (k is None and out_k is not None):
             raise ValueError("an output without its input")
+        if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, out_q, out_k)):
+            raise ValueError("apply is not recorded for autograd and would drop the gradient: call it under torch.no_grad(); "
+                             "the gradient of its inputs is apply(..., inverse=True) of the outputs'")
         if pos.dtype is not torch.int32 or pos.dim() != 1 or not pos.is_contiguous() or pos.get_device() != self.device:
             raise ValueError(f"pos must be a contiguous int32 vector on cuda:{self.device}")
         self._torch_dtype = torch.float16 if self.dtype == capi.F16 else torch.bfloat16
