@@ -429,11 +429,11 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
 #pragma unroll
             for (int k = 0; k < 4; k++) s[0][k] += s2[k];
         }
-        // s becomes the score in the log2 domain.  A K row whose byte is 0 (everything below 2^-118) counts as zeros.
+        // s becomes the score in the log2 domain
         float ev0 = 0.f, ev1 = 0.f, ks0 = 1.f, ks1 = 1.f;
         if (POOL8) {
-            ks0 = __uint_as_float(lds8(tile + 2 * TILE + g) << 23);
-            ks1 = __uint_as_float(lds8(tile + 2 * TILE + g + 8) << 23);
+            ks0 = __uint_as_float(max(lds8(tile + 2 * TILE + g) << 23, 0x00400000u));       // 2^(byte - 127), subnormal for 0
+            ks1 = __uint_as_float(max(lds8(tile + 2 * TILE + g + 8) << 23, 0x00400000u));
             ev0 = (float)lds8(tile + 2 * TILE + 16 + g);
             ev1 = (float)lds8(tile + 2 * TILE + 24 + g);
         }

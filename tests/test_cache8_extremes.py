@@ -186,3 +186,31 @@ def test_lists_over_one_vast_page(drkv_lib):
     want, pv, mag = R.attend(qd, kd, vd, 0.125)
     assert (np.abs(got - want) <= R.attend_tolerance(want, pv, mag, _half_step("f16"), 2.0 ** -21)).all()
     eng.close()
+
+
+def test_smallest_keys_and_large_queries(drkv_lib):
+    """Keys whose exponent byte is 0 (their row's largest is at most 448 * 2^-127) against queries that make scores of them."""
+    import torch
+    n, d = 40, 64
+    eng = _engine(hq=2, hkv=1, d=d, page=16, dtype="bf16", pages=8, seqs=1)
+    eng.seq_create()
+    assert eng.ensure_blocks_for_range(0, 0, n)
+    eng.set_seq_len(0, n)
+    eng.sync_block_table()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = (torch.randint(1, 28, (n, 1, d), generator=g, device="cuda") * 2.0 ** -126).bfloat16()
+    v = torch.randn(n, 1, d, generator=g, device="cuda").bfloat16()
+    q = (torch.randn(1, 2, d, generator=g, device="cuda") * 2.0 ** 119).bfloat16()
+    eng.append_rope_chunk(0, 0, 0, n, k, v)
+    kv_len = torch.full((1,), n, device="cuda", dtype=torch.int32)
+    out = torch.full_like(q, 7.0)
+    eng.attend_decode(0, 1, kv_len - n, kv_len, n, q, out, 0.25)
+    torch.cuda.synchronize()
+    e = R.quantise(k.double().cpu().numpy())[1]
+    assert (e == -127).all()
+    ks, vs = (R.stored_values(x.double().cpu().numpy())[:, 0] for x in (k, v))
+    want, pv, mag = R.attend(q[0].double().cpu().numpy(), ks, vs, 0.25)
+    assert (mag > 1).all()
+    err = np.abs(out[0].double().cpu().numpy() - want)
+    assert (err <= R.attend_tolerance(want, pv, mag, _half_step("bf16"), _weight_step("bf16"))).all()
+    eng.close()
