@@ -255,6 +255,7 @@ static BoundsParams bounds_params(drkv_engine* e, int layer) {
 // After kernels have written keys: one token of each batch entry (its position is d_pos + pos_offset) ...
 static int widen_batch(drkv_engine* e, int layer, int n, const int32_t* d_rows, const int32_t* d_pos, int pos_offset, cudaStream_t stream) {
     if (!e->bounds.on) return DRKV_OK;
+    DeviceGuard dev(e->device);
     BoundsParams p = bounds_params(e, layer);
     p.n_items = n;
     p.rows = d_rows;
@@ -266,6 +267,7 @@ static int widen_batch(drkv_engine* e, int layer, int n, const int32_t* d_rows, 
 // ... or tokens [pos_start, pos_start + m) of one sequence, in num_layers layers ...
 static int widen_range(drkv_engine* e, int layer, int num_layers, int row, int pos_start, int m, cudaStream_t stream) {
     if (!e->bounds.on || m <= 0) return DRKV_OK;
+    DeviceGuard dev(e->device);
     BoundsParams p = bounds_params(e, layer);
     const int P = e->geom.page_size;
     p.n_items = (int)(((int64_t)pos_start + m - 1) / P - pos_start / P + 1);
@@ -278,6 +280,7 @@ static int widen_range(drkv_engine* e, int layer, int num_layers, int row, int p
 // ... or whole pages, every layer and slot.
 static int rebuild_pages(drkv_engine* e, int page0, int n, cudaStream_t stream) {
     if (!e->bounds.on || n <= 0) return DRKV_OK;
+    DeviceGuard dev(e->device);
     BoundsParams p = bounds_params(e, 0);
     p.tables = nullptr;
     p.n_items = n;
@@ -304,6 +307,7 @@ static int run_cow(drkv_engine* e, const std::vector<CowJob>& jobs, cudaStream_t
     for (const CowJob& j : jobs) {
         e->cow_bytes += (int64_t)j.n_slots * e->geom.head_dim * 2 * (e->pool8 ? 1 : 2) * e->geom.num_kv_heads * e->geom.num_layers;
         if (!e->has_device) continue;
+        DeviceGuard dev(e->device);
         if (e->bounds.on)
             CUDA_TRY(launch_bounds_copy(bounds_params(e, 0), e->geom.head_dim, j.src_page, j.dst_page, e->geom.num_layers, stream));
         if (e->pool8) {
