@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kThreads8 = 256;
 constexpr int kMaxTokens8 = 128;  // tokens of one CTA of the append
-constexpr int kExpandCtas = 592;    // two waves of two an SM
 constexpr int kBatch8 = 4;        // rows a lane has in flight
 
 // Quantises the row of which each of its LANES lanes holds NV runs of 8 elements, runs l, l + LANES ...; row: its index in the
@@ -349,23 +348,23 @@ __global__ void __launch_bounds__(kThreads8) cow_copy8_kernel(const Pool8Layout 
 }
 
 template <template <typename, int> class Launch, typename P>
-cudaError_t by_shape(const P& p, int dtype, int head_dim, int n, cudaStream_t stream) {
+cudaError_t by_shape(const P& p, int dtype, int head_dim, int n, int num_sms, cudaStream_t stream) {
     const bool f16 = dtype == DRKV_DTYPE_F16;
     switch (head_dim) {
-        case 64: return f16 ? Launch<__half, 64>::run(p, n, stream) : Launch<__nv_bfloat16, 64>::run(p, n, stream);
-        case 128: return f16 ? Launch<__half, 128>::run(p, n, stream) : Launch<__nv_bfloat16, 128>::run(p, n, stream);
-        case 256: return f16 ? Launch<__half, 256>::run(p, n, stream) : Launch<__nv_bfloat16, 256>::run(p, n, stream);
+        case 64: return f16 ? Launch<__half, 64>::run(p, n, num_sms, stream) : Launch<__nv_bfloat16, 64>::run(p, n, num_sms, stream);
+        case 128: return f16 ? Launch<__half, 128>::run(p, n, num_sms, stream) : Launch<__nv_bfloat16, 128>::run(p, n, num_sms, stream);
+        case 256: return f16 ? Launch<__half, 256>::run(p, n, num_sms, stream) : Launch<__nv_bfloat16, 256>::run(p, n, num_sms, stream);
         default: return cudaErrorInvalidValue;
     }
 }
 template <typename T, int D>
 struct AppendLaunch {
-    static cudaError_t run(const Append8Params& p, int n, cudaStream_t s) {
+    static cudaError_t run(const Append8Params& p, int n, int num_sms, cudaStream_t s) {
         // A token a CTA for decode batches.  Tokens join while one wave of CTAs is left (4 of 256 threads an SM) until a lane
         // has two rows, the first to work on while the other comes, then up to six while there are two waves; their angles have
         // to fit 32 KB.  (4 097 tokens of 8 heads of 128, written and read: 11.5 us with two rows a lane, 13.0 with one.)
         constexpr int ROWS = kThreads8 / (D / (8 * kAppendRuns));
-        const int rows = 2 * p.layout.num_kv_heads, wave = 4 * 148;
+        const int rows = 2 * p.layout.num_kv_heads, wave = 4 * num_sms;
         int per = 1;
         while (per < kMaxTokens8 && 2 * per * p.rotary_dim <= 8192 &&
                ((per * rows < 2 * ROWS && n >= per * wave) || (per * rows < 6 * ROWS && n >= 2 * per * wave)))
@@ -377,49 +376,49 @@ struct AppendLaunch {
 // As many tokens a CTA as make one or two batches of rows a lane, fewer while the CTAs do not fill the SMs
 // (307 041 tokens of one head of 128 written and read: 83 us so, 110 with 16 a CTA; 1 592 tokens of 5 of 256: 7.8 and 8.4).
 template <typename T, int D, bool TO_FLAT>
-cudaError_t launch_flat8(const Flat8Params& p, cudaStream_t s) {
+cudaError_t launch_flat8(const Flat8Params& p, int num_sms, cudaStream_t s) {
     constexpr int ROWS = kThreads8 / (D / 8);
     const int H = p.layout.num_kv_heads;
     int per = kFlatTokens;
     while (per > 1 && per * H >= 2 * kBatch8 * ROWS) per /= 2;
-    while (per > 1 && (int64_t)((p.num_tokens + per - 1) / per) * 2 * p.num_layers < 4 * 148) per /= 2;
+    while (per > 1 && (int64_t)((p.num_tokens + per - 1) / per) * 2 * p.num_layers < 4 * num_sms) per /= 2;
     return launch_pdl(flat_copy8_kernel<T, D, TO_FLAT>, dim3((p.num_tokens + per - 1) / per, 2 * p.num_layers), dim3(kThreads8), 0, s, p, per,
                       magic_of(H));
 }
 template <typename T, int D>
 struct ExtractLaunch {
-    static cudaError_t run(const Flat8Params& p, int, cudaStream_t s) { return launch_flat8<T, D, true>(p, s); }
+    static cudaError_t run(const Flat8Params& p, int, int num_sms, cudaStream_t s) { return launch_flat8<T, D, true>(p, num_sms, s); }
 };
 template <typename T, int D>
 struct InjectLaunch {
-    static cudaError_t run(const Flat8Params& p, int, cudaStream_t s) { return launch_flat8<T, D, false>(p, s); }
+    static cudaError_t run(const Flat8Params& p, int, int num_sms, cudaStream_t s) { return launch_flat8<T, D, false>(p, num_sms, s); }
 };
 template <typename T, int D>
 struct ExpandLaunch {
-    static cudaError_t run(const Expand8Params& p, int n, cudaStream_t s) {
-        // Parts of one batch while the pages are few (one page of 128 tokens of 5 heads of 256: a 43-token chunk takes
+    static cudaError_t run(const Expand8Params& p, int n, int num_sms, cudaStream_t s) {
+        // Parts of one batch while the CTAs are fewer than two waves of two an SM (one page of 128 tokens of 5 heads of 256: a 43-token chunk takes
         // 51 us in one part, 13 in forty).
         const int batches = (2 * p.layout.num_kv_heads * p.layout.page_size * (D / 8) + kBatch8 * kThreads8 - 1) / (kBatch8 * kThreads8);
-        const int parts = min(batches, max(1, kExpandCtas / (n * p.n_seq)));
+        const int parts = min(batches, max(1, 4 * num_sms / (n * p.n_seq)));
         return launch_pdl(expand8_kernel<T, D>, dim3(n, p.n_seq, parts), dim3(kThreads8), 0, s, p);
     }
 };
 
 }  // namespace
 
-cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, cudaStream_t stream) {
+cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, int num_sms, cudaStream_t stream) {
     if (n_tokens <= 0) return cudaSuccess;
-    return by_shape<AppendLaunch>(p, dtype, p.layout.head_dim, n_tokens, stream);
+    return by_shape<AppendLaunch>(p, dtype, p.layout.head_dim, n_tokens, num_sms, stream);
 }
 
-cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, cudaStream_t stream) {
+cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, int num_sms, cudaStream_t stream) {
     if (p.num_tokens <= 0) return cudaSuccess;
     if (p.num_layers > 32767) return cudaErrorInvalidValue;          // grid.y
-    return to_flat ? by_shape<ExtractLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, stream)
-                   : by_shape<InjectLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, stream);
+    return to_flat ? by_shape<ExtractLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, num_sms, stream)
+                   : by_shape<InjectLaunch>(p, dtype, p.layout.head_dim, p.num_tokens, num_sms, stream);
 }
 
-cudaError_t launch_expand8(const Expand8Params& p, int dtype, cudaStream_t stream) {
+cudaError_t launch_expand8(const Expand8Params& p, int dtype, int num_sms, cudaStream_t stream) {
     int pages = 0;
     for (int i = 0; i < p.n_seq; i++) {
         const int n = (int)(((int64_t)p.n_tokens[i] + p.layout.page_size - 1) / p.layout.page_size);
@@ -427,7 +426,7 @@ cudaError_t launch_expand8(const Expand8Params& p, int dtype, cudaStream_t strea
     }
     if (pages > p.table_stride) pages = p.table_stride;
     if (pages <= 0) return cudaSuccess;
-    return by_shape<ExpandLaunch>(p, dtype, p.layout.head_dim, pages, stream);
+    return by_shape<ExpandLaunch>(p, dtype, p.layout.head_dim, pages, num_sms, stream);
 }
 
 cudaError_t launch_cow_copy8(const Pool8Layout& layout, uint8_t* pool, int src_page, int dst_page, int num_layers, cudaStream_t stream) {

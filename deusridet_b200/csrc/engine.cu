@@ -261,7 +261,7 @@ static int widen_batch(drkv_engine* e, int layer, int n, const int32_t* d_rows, 
     p.rows = d_rows;
     p.pos = d_pos;
     p.pos_offset = pos_offset;
-    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), 1, stream));
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), 1, e->num_sms, stream));
     return DRKV_OK;
 }
 // ... or tokens [pos_start, pos_start + m) of one sequence, in num_layers layers ...
@@ -274,7 +274,7 @@ static int widen_range(drkv_engine* e, int layer, int num_layers, int row, int p
     p.row = row;
     p.pos_start = pos_start;
     p.m = m;
-    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), num_layers, stream));
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), num_layers, e->num_sms, stream));
     return DRKV_OK;
 }
 // ... or whole pages, every layer and slot.
@@ -285,7 +285,7 @@ static int rebuild_pages(drkv_engine* e, int page0, int n, cudaStream_t stream) 
     p.tables = nullptr;
     p.n_items = n;
     p.page0 = page0;
-    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), e->geom.num_layers, stream));
+    CUDA_TRY(launch_bounds(p, e->pool8, e->geom.head_dim, io_dtype(e->geom), e->geom.num_layers, e->num_sms, stream));
     return DRKV_OK;
 }
 // Pages that came back from the storage tier get their bounds anew (all of a page's slots: a partly filled page's bounds
@@ -871,7 +871,7 @@ static int append8(drkv_engine* e, int layer, int n, const int32_t* d_rows, cons
     p.inv_freq = e->d_inv_freq;
     p.k_src = k_src;
     p.v_src = v_src;
-    CUDA_TRY(launch_append8(p, n, io_dtype(e->geom), stream));
+    CUDA_TRY(launch_append8(p, n, io_dtype(e->geom), e->num_sms, stream));
     return DRKV_OK;
 }
 
@@ -941,7 +941,7 @@ static int seq_flat_copy(drkv_engine* e, int seq, int start_token, int num_token
         f.start_token = start_token;
         f.num_tokens = num_tokens;
         f.num_layers = e->geom.num_layers;
-        CUDA_TRY(launch_flat_copy8(f, to_flat, io_dtype(e->geom), (cudaStream_t)stream));
+        CUDA_TRY(launch_flat_copy8(f, to_flat, io_dtype(e->geom), e->num_sms, (cudaStream_t)stream));
         return to_flat ? DRKV_OK : widen_range(e, 0, e->geom.num_layers, seq, start_token, num_tokens, (cudaStream_t)stream);
     }
     FlatCopyParams p{};
@@ -1884,7 +1884,7 @@ int drkv_attend_prefill_batch(drkv_engine* e, int layer, int n_seq, const int32_
                 x.row[i] = p.row[i];
                 x.n_tokens[i] = p.m[i] == 0 ? 0 : p.m[i] > INT32_MAX - p.pos_start[i] ? INT32_MAX : p.pos_start[i] + p.m[i];
             }
-            CUDA_TRY(launch_expand8(x, io_dtype(g), (cudaStream_t)stream));
+            CUDA_TRY(launch_expand8(x, io_dtype(g), e->num_sms, (cudaStream_t)stream));
             p.layer = 0;
         }
         p.max_pages = e->book.max_pages();

@@ -161,7 +161,7 @@ struct Append8Params {
     const void* k_src;
     const void* v_src;
 };
-cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, cudaStream_t stream);
+cudaError_t launch_append8(const Append8Params& p, int n_tokens, int dtype, int num_sms, cudaStream_t stream);
 
 struct Flat8Params {
     Pool8Layout layout;
@@ -170,7 +170,7 @@ struct Flat8Params {
     const int32_t* table;
     int table_stride, start_token, num_tokens, num_layers;
 };
-cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, cudaStream_t stream);
+cudaError_t launch_flat_copy8(const Flat8Params& p, bool to_flat, int dtype, int num_sms, cudaStream_t stream);
 
 // Pages of up to kMaxPrefillSeqs sequences expanded into a 16-bit image of one layer with the same page ids.
 struct Expand8Params {
@@ -181,7 +181,7 @@ struct Expand8Params {
     int table_stride, layer, n_seq;
     int row[kMaxPrefillSeqs], n_tokens[kMaxPrefillSeqs];
 };
-cudaError_t launch_expand8(const Expand8Params& p, int dtype, cudaStream_t stream);
+cudaError_t launch_expand8(const Expand8Params& p, int dtype, int num_sms, cudaStream_t stream);
 cudaError_t launch_cow_copy8(const Pool8Layout& layout, uint8_t* pool, int src_page, int dst_page, int num_layers, cudaStream_t stream);
 
 // ---- decode attention over the 8-bit pool, and over listed pages of either pool (attend_pages.cu) ----
@@ -222,7 +222,7 @@ struct BoundsParams {
     int row, pos_start, m;    // range of one sequence (tables != nullptr, rows == nullptr)
     int page0;                // pages (tables == nullptr)
 };
-cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, cudaStream_t stream);
+cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, int num_sms, cudaStream_t stream);
 cudaError_t launch_bounds_copy(const BoundsParams& p, int head_dim, int src_page, int dst_page, int num_layers, cudaStream_t stream);
 struct SelectParams {
     const int8_t* bounds;

@@ -607,10 +607,10 @@ cudaError_t launch_score(const SelectParams& p, int num_sms, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, cudaStream_t stream) {
+cudaError_t launch_bounds(const BoundsParams& p, bool pool8, int head_dim, int dtype, int num_layers, int num_sms, cudaStream_t stream) {
     if (p.n_items <= 0 || num_layers <= 0) return cudaSuccess;
     const int64_t items = (int64_t)p.n_items * p.num_kv_heads;
-    const bool split = p.rows == nullptr && items * num_layers < 64 * 148;   // 64 warps an SM
+    const bool split = p.rows == nullptr && items * num_layers < 64 * num_sms;   // 64 warps an SM
     const int64_t blocks = split ? items : (items + 7) / 8;
     if (blocks > 0x7fffffff || num_layers > 65535) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)blocks, num_layers);
