@@ -299,6 +299,7 @@ DRKV_API const int8_t* drkv_page_bound_exponents(const drkv_engine* e);
  * top_pages of them; else the first first_pages and the last last_pages logical pages (where resident) and the best scored
  * (ties: the lower page).  With q8_h = rint(q_h / 2^f), f the smallest integer with max|q_h| <= 127 * 2^f, a page's score is the
  * largest over the KV head's query heads of 2^(e + f) * sum_d (q8[d] > 0 ? q8[d] * b_max[d] : q8[d] * b_min[d]).
+ * The sums are exact; scores are compared as fp32 numbers, so those beyond fp32's range are equal (infinite, or 0).
  * q, d_rows, d_kv_len and max_kv_len as in drkv_attend_decode; first_pages + last_pages <= top_pages. */
 DRKV_API int drkv_select_pages(drkv_engine* e, int layer, int n_seq, const int32_t* d_rows, const int32_t* d_kv_len,
                                int max_kv_len, const void* q, int top_pages, int first_pages, int last_pages, int32_t* d_sel,
