@@ -13,6 +13,7 @@ public:
             ok_ = cudaSetDevice(device) == cudaSuccess;
             changed_ = ok_;
         }
+        if (!ok_) cudaGetLastError();   // reported by ok(): not left behind for the caller's next CUDA call
     }
     ~DeviceGuard() {
         if (changed_) cudaSetDevice(prev_);

@@ -1914,6 +1914,7 @@ int drkv_page_bounds_enable(drkv_engine* e, void* stream) {
         if (ce == cudaSuccess) ce = cudaMalloc(&x, n);
         if (ce != cudaSuccess) {
             cudaFree(b);
+            cudaGetLastError();                  // reported here, not left for the caller's next CUDA call
             return set_err(DRKV_ERR_CUDA, "page_bounds_enable: %s", cudaGetErrorString(ce));
         }
         e->bounds.d_bounds = b;

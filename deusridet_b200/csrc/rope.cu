@@ -442,6 +442,7 @@ int drkv_rope_create(const drkv_rope_config* cfg, drkv_rope** out) {
             cudaMalloc(&r->d_turns, turns.size() * 8) != cudaSuccess ||
             cudaMemcpy(r->d_turns, turns.data(), turns.size() * 8, cudaMemcpyHostToDevice) != cudaSuccess) {
             cudaFree(r->d_turns);
+            cudaGetLastError();          // reported here
             delete r;
             return fail(DRKV_ERR_CUDA, "rope_create: allocating the frequency table failed");
         }
