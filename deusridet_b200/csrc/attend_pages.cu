@@ -27,11 +27,15 @@
 // are 2^((s - m) + (ev - E) + 7), at most 2^15 since they may pass the reference by 2^8 before it follows, of full precision
 // down to 2^-20 of the largest, and vanish below 2^-31 of it: next to what the same head has summed, whatever the sizes of
 // rows that hold no weight.  o carries 2^E, in the pieces too; the sum of the weights stays relative to m, in fp32.
-// (A second exponential and two additions per key and head: 64 sequences, 109.8 us a step with them and without.)
+// (A second exponential and two additions per key and head, measured with one term of P: 64 sequences, 108 us a step with
+// them and 109 without; of heads of 64 dims, where a group is half as long, 67 and 66.)
 // bf16 queries are scaled by a power of two per head into f16 (8 significant bits fit; exact unless an element is below
 // 2^-27 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
-// P in the PV product: f16 hi + lo terms (22 bits) over an 8-bit or an f16 pool, bf16 hi + lo (16 bits) over a bf16 pool.  (One
-// f16 term for bf16 outputs of the 8-bit pool took as long: 109.8 us for 64 sequences with one, 108.7 with two.)
+// P in the PV product: f16 hi + lo terms (22 bits) over an 8-bit or an f16 pool, bf16 hi + lo (16 bits) over a bf16 pool.  Only
+// bf16 outputs of groups beyond eight heads over the 8-bit pool have one f16 term (2^-12 of a weight beside the output's 2^-9):
+// with two column tiles the products count, and 64 sequences of 128 heads take 156 us with two terms, 139 with one.  (Of 32
+// heads 113 and 108, of 64 dims 70 and 67, in a loop of seconds, at the 1.65 GHz that the power cap leaves; in a short one, at
+// full clock, 108 either way.)
 #include <atomic>
 
 #include "kernels.hpp"
@@ -114,6 +118,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
     constexpr int WARPS = Ring<POOL8, D, NQ>::kWarps, STAGES = Ring<POOL8, D, NQ>::kStages, THREADS = WARPS * 32;
     using TM = typename std::conditional<POOL8, __half, T>::type;           // matrix operand type
     constexpr bool F16 = std::is_same<TM, __half>::value;
+    constexpr bool LO = !(POOL8 && std::is_same<T, __nv_bfloat16>::value && NQ == 2);
     constexpr int ROWB = D * (POOL8 ? 1 : 2), CPR = ROWB / 16, TILE = 16 * ROWB;
     constexpr int SLOT = 2 * TILE + (POOL8 ? 32 : 0);
     constexpr int KSTEPS = D / 16, MT = D / 16;
@@ -281,7 +286,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
     uint32_t qf[NQ][KSTEPS][2];
     float qs[NQ][2];                                                        // score factor of heads 2t and 2t + 1
     float o[NQ][MT][4], m[NQ][2], l[NQ][2];
-    float lift[NQ][2];                                                      // 8-bit pool: WS - E, E in exponent bytes, whole
+    float big_e[NQ][2];                                                     // 8-bit pool: E, an exponent byte
     int cur_pair = -1;
 
     auto begin_pair = [&](int pair) {
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             qs[nq][1] = __shfl_sync(FULL, own_scale, 8 * t + 4);
             m[nq][0] = m[nq][1] = kNoKey;
             l[nq][0] = l[nq][1] = 0.f;
-            lift[nq][0] = lift[nq][1] = WS;
+            big_e[nq][0] = big_e[nq][1] = 0.f;
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) o[nq][mt][0] = o[nq][mt][1] = o[nq][mt][2] = o[nq][mt][3] = 0.f;
         }
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                 const int head = nq * 8 + 2 * t + c;
                 if (head < p.group) {
                     const float f = (whole ? 1.f / sum : 1.f) * (F16 ? 0x1p-7f : 1.f);
-                    const float e = POOL8 ? WS - lift[nq][c] : 127.f, unit = whole ? exp2_int((int)e - 127) : 1.f;
+                    const float e = POOL8 ? big_e[nq][c] : 127.f, unit = whole ? exp2_int((int)e - 127) : 1.f;
                     if (!whole && g == 0) pieces.mle[row0 + head] = make_float4(m[nq][c], sum, e, 0.f);
 #pragma unroll
                     for (int j = 0; j < VCH; j++) {
@@ -434,16 +439,20 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
         if (POOL8) {
             ks0 = __uint_as_float(max(lds8(tile + 2 * TILE + g) << 23, 0x00400000u));       // 2^(byte - 127), subnormal for 0
             ks1 = __uint_as_float(max(lds8(tile + 2 * TILE + g + 8) << 23, 0x00400000u));
-            ev0 = (float)lds8(tile + 2 * TILE + 16 + g);
-            ev1 = (float)lds8(tile + 2 * TILE + 24 + g);
+            // byte + WS: the byte as the lowest bits of 2^23
+            ev0 = __uint_as_float(0x4b000000u | lds8(tile + 2 * TILE + 16 + g)) - (8388608.f - WS);
+            ev1 = __uint_as_float(0x4b000000u | lds8(tile + 2 * TILE + 24 + g)) - (8388608.f - WS);
         }
         if (valid < 16) {                                                   // what lies behind the last key may be anything
             if (g >= valid) ev0 = ks0 = 0.f;
             if (g + 8 >= valid) ev1 = ks1 = 0.f;
         }
-        // The maximum and the weights' reference follow only when a score exceeds one of them by more than kSlack, and then
-        // in full: most groups need no reduction over the lanes.
-        bool grow = false;
+        // The maximum and the weights' reference follow only when a score exceeds one of them by more than the slack, and then
+        // in full: most groups need no reduction over the lanes.  (Over the 8-bit pool p goes into a sum in fp32 alone, and
+        // may pass its maximum by as much as the weights' exponents show.)
+        constexpr float LIMIT = POOL8 ? kSlack + WS : kSlack;
+        float t0[NQ][2], t1[NQ][2], y0[NQ][2], y1[NQ][2];                   // binary logarithms of p and, with 2^WS, of the weight
+        float over = -INFINITY;
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++)
 #pragma unroll
@@ -453,15 +462,16 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                 // product's lower half alone could exceed the slack
                 s[nq][c] = __fmul_rn(s[nq][c], f0);
                 s[nq][2 + c] = __fmul_rn(s[nq][2 + c], f1);
+                t0[nq][c] = __fadd_rn(s[nq][c], -m[nq][c]);
+                t1[nq][c] = __fadd_rn(s[nq][2 + c], -m[nq][c]);
+                over = fmax3(over, t0[nq][c], t1[nq][c]);
                 if (POOL8) {
-                    const float t0 = __fadd_rn(s[nq][c], -m[nq][c]), t1 = __fadd_rn(s[nq][2 + c], -m[nq][c]);
-                    grow |= fmaxf(t0, t1) > kSlack;
-                    grow |= fmaxf(t0 + (ev0 + lift[nq][c]), t1 + (ev1 + lift[nq][c])) > kSlack + WS;
-                } else {
-                    grow |= __fadd_rn(fmaxf(s[nq][c], s[nq][2 + c]), -m[nq][c]) > kSlack;
+                    y0[nq][c] = t0[nq][c] + (ev0 - big_e[nq][c]);
+                    y1[nq][c] = t1[nq][c] + (ev1 - big_e[nq][c]);
+                    over = fmax3(over, y0[nq][c], y1[nq][c]);
                 }
             }
-        if (__any_sync(FULL, grow)) {
+        if (__any_sync(FULL, over > LIMIT)) {
             auto over_keys = [&](float a, float b) -> float {               // maximum over the group's visible keys
                 float x = fmaxf(g < valid ? a : -INFINITY, g + 8 < valid ? b : -INFINITY);
                 x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
@@ -477,12 +487,16 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
                     float r = f;
                     if (POOL8) {
                         // whole, so that o's unit stays a power of two; never above the largest exponent byte met
-                        const float seen = over_keys((s[nq][c] - x) + ev0, (s[nq][2 + c] - x) + ev1), old = WS - lift[nq][c];
+                        const float seen = over_keys((s[nq][c] - x) + ev0, (s[nq][2 + c] - x) + ev1) - WS, old = big_e[nq][c];
                         const float e = whole_byte(fmaxf(seen, down + old));
                         r = fast_exp2(down + (old - e));
-                        lift[nq][c] = WS - e;
+                        big_e[nq][c] = e;
                     }
                     m[nq][c] = x;
+                    t0[nq][c] = __fadd_rn(s[nq][c], -x);
+                    t1[nq][c] = __fadd_rn(s[nq][2 + c], -x);
+                    y0[nq][c] = t0[nq][c] + (ev0 - big_e[nq][c]);
+                    y1[nq][c] = t1[nq][c] + (ev1 - big_e[nq][c]);
                     l[nq][c] *= f;
 #pragma unroll
                     for (int mt = 0; mt < MT; mt++) {
@@ -495,25 +509,34 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
         uint32_t pf[NQ][2], pl[NQ][2];
 #pragma unroll
         for (int nq = 0; nq < NQ; nq++) {
-            float w0[2], w1[2];
+            float p0[2], p1[2], w0[2], w1[2];
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const float t0 = __fadd_rn(s[nq][c], -m[nq][c]), t1 = __fadd_rn(s[nq][2 + c], -m[nq][c]);
-                const float p0 = fast_exp2(t0), p1 = fast_exp2(t1);
-                l[nq][c] += (g < valid ? p0 : 0.f) + (g + 8 < valid ? p1 : 0.f);
-                w0[c] = POOL8 ? fast_exp2(t0 + (ev0 + lift[nq][c])) : F16 ? p0 * 0x1p7f : p0;
-                w1[c] = POOL8 ? fast_exp2(t1 + (ev1 + lift[nq][c])) : F16 ? p1 * 0x1p7f : p1;
+                p0[c] = fast_exp2(t0[nq][c]);
+                p1[c] = fast_exp2(t1[nq][c]);
+                w0[c] = POOL8 ? fast_exp2(y0[nq][c]) : p0[c];
+                w1[c] = POOL8 ? fast_exp2(y1[nq][c]) : p1[c];
             }
             if (valid < 16) {
-                if (g >= valid) w0[0] = w0[1] = 0.f;
-                if (g + 8 >= valid) w1[0] = w1[1] = 0.f;
+                if (g >= valid) p0[0] = p0[1] = w0[0] = w0[1] = 0.f;
+                if (g + 8 >= valid) p1[0] = p1[1] = w1[0] = w1[1] = 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                l[nq][c] += p0[c] + p1[c];
+                if (!POOL8 && F16) {
+                    w0[c] *= 0x1p7f;
+                    w1[c] *= 0x1p7f;
+                }
             }
             const uint32_t h0 = Elem<TM>::pack2(w0[0], w0[1]), h1 = Elem<TM>::pack2(w1[0], w1[1]);
             pf[nq][0] = transpose8x8(h0);
             pf[nq][1] = transpose8x8(h1);
-            const float2 a = Elem<TM>::unpack2(h0), b = Elem<TM>::unpack2(h1);
-            pl[nq][0] = transpose8x8(Elem<TM>::pack2(w0[0] - a.x, w0[1] - a.y));
-            pl[nq][1] = transpose8x8(Elem<TM>::pack2(w1[0] - b.x, w1[1] - b.y));
+            if (LO) {
+                const float2 a = Elem<TM>::unpack2(h0), b = Elem<TM>::unpack2(h1);
+                pl[nq][0] = transpose8x8(Elem<TM>::pack2(w0[0] - a.x, w0[1] - a.y));
+                pl[nq][1] = transpose8x8(Elem<TM>::pack2(w1[0] - b.x, w1[1] - b.y));
+            }
         }
         // ---- O^T += V^T P^T: keys 2t, 2t + 1, 2t + 8, 2t + 9; dims (g + 8 j) EPL + 0 .. EPL - 1 ----
         const uint32_t vt = tile + TILE;
@@ -521,7 +544,7 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
 #pragma unroll
             for (int nq = 0; nq < NQ; nq++) {
                 mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pf[nq][0], pf[nq][1]);
-                mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pl[nq][0], pl[nq][1]);
+                if (LO) mma16816<TM>(o[nq][mt], a0, a1, a2, a3, pl[nq][0], pl[nq][1]);
             }
         };
 #pragma unroll
