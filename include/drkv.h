@@ -58,6 +58,12 @@ typedef enum drkv_status {
  * x * 2^-e rounded to e4m3 (nearest even); it stands for those values times 2^e.  Infinities saturate, NaN stays NaN, and
  * neither counts towards the maximum; K is rotated in fp32 before it is rounded.  drkv_seq_extract returns the values
  * rounded to Q's type, which holds them exactly except below fp16's steps and beyond its range.  No counterpart in the reference.
+ * Decode attention takes the stored values as they are and the softmax weights in 22 bits (12 for a bf16 Q with more than eight
+ * query heads a KV head); of a bf16 query row, elements below 2^-30 of the largest may lose bits.  Prefill attention is that of
+ * a 16-bit pool holding what drkv_seq_extract returns: weights rounded to Q's type, and with an fp16 Q the values' rounding too,
+ * so that prefill and decode of one cache may differ by it.
+ * Beside the pool, and outside drkv_config.budget_bytes, an 8-bit engine allocates at creation what its prefill reads, one layer
+ * in 16 bits: 4 * num_kv_heads * page_size * head_dim bytes a page, close to twice the pool's bytes per layer.
  * With an 8-bit pool the planned decode pass reads every sequence by itself, and these calls are refused
  * (DRKV_ERR_INVALID): drkv_attend_partial, drkv_exchange_create, drkv_scorer_enable, drkv_set_prefill_on_decode_kernel(1)
  * and the raw-pointer drkv_k_* functions. */
