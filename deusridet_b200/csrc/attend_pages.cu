@@ -10,9 +10,10 @@
 // stretch is finished by its warp; one that is cut leaves a piece (m, l, o) per stretch, at most two a warp, and a second
 // small kernel merges them in a fixed order (results do not depend on timing).  Warps of one CTA take stretches far apart,
 // so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and then by the last CTA to arrive, took
-// 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end.
-// Bound by HBM: the loop over groups reads 7 TB/s (131 001 keys of 8 heads, 270 MB: 50 us, 5 more for the merge; 64 sequences
-// of 1-8 k keys, 602 MB: 106 us and 4); what is left is the first data of a launch, the uneven finish and the merge.
+// 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end (not measured on short lines).
+// Bound by HBM: from 131 001 to 524 001 keys of 8 heads of 128 a key more costs its bytes at 6.1 to 6.4 TB/s (54 and 183 us with
+// the merge; at 5.7 in a loop of seconds, where the power cap leaves 1.6 GHz), beside a fixed 10 us for the first data, the
+// uneven finish and the merge.  64 sequences of 1-8 k keys, 602 MB: 106 us, 5.7 TB/s.
 //
 // A warp brings its groups into a private ring of shared memory by cp.async (16 bytes a lane, L1 bypassed), kStages - 1
 // groups ahead, and reads them as matrix operands without ldmatrix: contraction order is free, so a lane takes whole
@@ -30,7 +31,7 @@
 // (A second exponential and two additions per key and head, measured with one term of P: 64 sequences, 108 us a step with
 // them and 109 without; of heads of 64 dims, where a group is half as long, 67 and 66.)
 // bf16 queries are scaled by a power of two per head into f16 (8 significant bits fit; exact unless an element is below
-// 2^-27 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
+// 2^-30 of its row's maximum).  Scores, maxima, sums and outputs accumulate in fp32.
 // P in the PV product: f16 hi + lo terms (22 bits) over an 8-bit or an f16 pool, bf16 hi + lo (16 bits) over a bf16 pool.  Only
 // bf16 outputs of groups beyond eight heads over the 8-bit pool have one f16 term (2^-12 of a weight beside the output's 2^-9):
 // with two column tiles the products count, and 64 sequences of 128 heads take 156 us with two terms, 139 with one.  (Of 32

@@ -9,8 +9,10 @@
 // order and on every unit, so equal scores are equal bits and the selection is reproducible (ties: lowest page).
 // As a contraction: [q8 clipped to >= 0, q8 clipped to <= 0] . [b_max, b_min], 2 D long, on int8 mma.sync tiles.
 //
-// The score pass reads 2 D + 1 bytes per page and KV head where the page's K and V rows are 4 P D in 16 bits: HBM-bound for
-// long contexts; the selection runs on the scores in shared memory, one CTA per (sequence, KV head).
+// The score pass reads 2 D + 1 bytes per page and KV head where the page's K and V rows are 4 P D in 16 bits.  86 MB take it
+// 20 us, 4.3 TB/s with DRAM 46 % and the issue slots 48 % busy: bound by the latency of a warp's 32 to 64 pages, two to four
+// stages behind the making of its query bytes.  The selection runs on the scores in shared memory, one CTA per (sequence, KV
+// head): a chain of scans, latency too.
 #include <atomic>
 
 #include "kernels.hpp"
