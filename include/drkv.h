@@ -63,7 +63,8 @@ typedef enum drkv_status {
  * a 16-bit pool holding what drkv_seq_extract returns: weights rounded to Q's type, and with an fp16 Q the values' rounding too,
  * so that prefill and decode of one cache may differ by it.
  * Beside the pool, and outside drkv_config.budget_bytes, an 8-bit engine allocates at creation what its prefill reads, one layer
- * in 16 bits: 4 * num_kv_heads * page_size * head_dim bytes a page, close to twice the pool's bytes per layer.
+ * in 16 bits: 4 * num_kv_heads * page_size * head_dim bytes a page, close to twice the pool's bytes per layer.  A layer of 2^31
+ * K and V rows or more has no prefill (DRKV_ERR_CAPACITY).
  * With an 8-bit pool the planned decode pass reads every sequence by itself, and these calls are refused
  * (DRKV_ERR_INVALID): drkv_attend_partial, drkv_exchange_create, drkv_scorer_enable, drkv_set_prefill_on_decode_kernel(1)
  * and the raw-pointer drkv_k_* functions. */

@@ -1,4 +1,4 @@
-"""Rope.apply and autograd: nothing that requires a gradient goes through it unnoticed."""
+"""What Rope refuses besides sizes: tensors that require a gradient, devices that are not there."""
 import pytest
 
 
