@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(Ring<POOL8, D, NQ>::kWarps * 32, 1) attend_pag
             const int i = lo + idx - s.start;
             ahead_logical = i / per_page;
             ahead_in = i - ahead_logical * per_page;
-            if (LIST) ahead_logical = __ldg(p.list + (int64_t)s.pair * p.list_len + ahead_logical);
+            // (a plain load: the kernel in front may have written the list while this one was already running)
+            if (LIST) ahead_logical = p.list[(int64_t)s.pair * p.list_len + ahead_logical];
         }
     };
     auto locate_page = [&]() {                                              // step 2: page

@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kThreads8) expand8_kernel(const Expand8Params 
             e[u] = 0;
             if (i < total) {
                 q[u] = __ldcs(reinterpret_cast<const uint2*>(block) + i);
-                e[u] = __ldg(exps + r);
+                e[u] = exps[r];                                      // (a plain load: the kernel in front may have written it)
             }
         }
 #pragma unroll

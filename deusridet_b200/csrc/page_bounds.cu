@@ -254,7 +254,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32) page_score_kernel(const Sele
         }
         return page;
     };
-    auto exponent_of = [&](int page) -> int { return page >= 0 ? __ldg(p.exponents + (layer0 + page) * p.num_kv_heads + h) : 0; };
+    // (a plain load: the kernel in front may have written them while this one was already running)
+    auto exponent_of = [&](int page) -> int { return page >= 0 ? p.exponents[(layer0 + page) * p.num_kv_heads + h] : 0; };
     iss32 = checked(iss32);
     iss_next = checked(iss_next);
     int page32 = iss32, next32 = iss_next;                                  // of the window being scored, and the one behind it
