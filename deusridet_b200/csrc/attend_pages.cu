@@ -6,8 +6,8 @@
 //
 // Split: the keys of all (sequence, KV head) pairs form one line of 16-key groups.  Every warp of a persistent grid takes
 // an equal stretch of it, whatever the lengths are: ragged batches need no queue and no tail, and short lines are spread as
-// far as they go (1500 keys of 4 heads: 11.3 us a step with one group a warp, 14.0 with four).  A pair that lies inside one
-// stretch is finished by its warp; one that is cut leaves a piece (m, l, o) per stretch, at most two a warp, and a second
+// far as they go (1500 keys of 4 heads: 10.4 us a step with one group a warp, 13.5 with four).  A pair that lies inside one
+// stretch is finished by its warp; one that is cut leaves a piece (m, l, E, o) per stretch, at most two a warp, and a second
 // small kernel merges them in a fixed order (results do not depend on timing).  Warps of one CTA take stretches far apart,
 // so that a short line still spreads over all SMs.  Merging inside the kernel, by CTA and then by the last CTA to arrive, took
 // 9 us longer on 131 000 keys: fences and a chain of loads by a few CTAs at the end (not measured on short lines).
