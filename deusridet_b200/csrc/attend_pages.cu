@@ -735,7 +735,7 @@ cudaError_t launch_one(const AttendPagesParams& p, int num_sms, cudaStream_t str
     const int64_t pairs = (int64_t)p.n_seq * p.num_kv_heads, rows = pairs * p.group;
     // About n_warps / pairs pieces a row, eight of which a set of lanes takes at a time: the more pieces, the fewer dims a CTA
     // takes and the more sets it has (60 rows of 118 pieces of 256 dims: 20 us a pass with four sets, 15 with thirty-two), as
-    // long as the CTAs are resident in two turns (3 360 rows of 9 pieces of 64 dims, a CTA each: 43 us a pass; eight a CTA: 21).
+    // long as the CTAs are resident in two turns (3 360 rows of 9 pieces of 64 dims, a CTA each: 43 us a pass; eight a CTA: 22).
     const int64_t pieces = n_warps / pairs + 2, most = 4 * (int64_t)num_sms;
     if (pieces > 8 && rows <= most) {
         constexpr int MID = D > 64 ? 64 : D;
